@@ -232,6 +232,113 @@ int mxk_linear_bf16(const mxk_bf16* A, const mxk_bf16* W, const float* bias, int
 int mxk_linear_gated_residual(const mxk_bf16* A, const mxk_bf16* W, const float* bias, int64_t M, int64_t N, int64_t K, float* x,
                               MxkRowMod gate, int gate_tanh, mxk_stream_t stream);
 
+/* ---- paged key/value cache and attention ------------------------------------------------
+ * No counterpart in the reference's ops.h: its attention (src/kernels/attention.h:21-39) takes one dense segment per
+ * call and keeps no cache.  These take what mxk_qkv_norm_rope and the linear layers produce ([rows, heads, D] bf16,
+ * packed or not) and write the input of the attention out-projection.  Forward only, like everything else here.
+ *
+ * MxkKvCache describes a cache that several calls share: `k` and `v` are num_pages pages of page_size tokens of Hkv
+ * heads of D channels; element (page, slot, head, channel) of either is at page * page_stride + slot * token_stride +
+ * head * head_stride + channel (strides in elements, so both [page, slot, head, D] and [page, head, slot, D] are
+ * covered; all multiples of 16 bytes, k and v 16-byte aligned).  Token t of sequence b is slot t % page_size of page
+ * page_table[b * table_stride + t / page_size]; a sequence has room for max_pages * page_size tokens.  The same page
+ * may stand in several rows of the table (a shared prefix).
+ * type MXK_KV_BF16: bf16 values.  MXK_KV_E4M3: fp8 e4m3 values, element = value / scale rounded to nearest, ties to
+ * even, saturating at +-448; k_scale / v_scale fp32 [Hkv] or NULL (1).
+ * Page numbers, sequence numbers, positions and lengths are read on the device.  One that is out of range is never
+ * followed: the row or token is left out and mxk_device_error() reports MXK_DEVICE_ERR_BAD_INDEX. */
+#define MXK_KV_BF16 0
+#define MXK_KV_E4M3 1
+#define MXK_DEVICE_ERR_BAD_INDEX 2
+#define MXK_ATTN_MAX_HEAD_DIM 128
+typedef struct MxkKvCache {
+  void* k;
+  void* v;
+  const int32_t* page_table; /* [n_seqs, max_pages], rows table_stride apart */
+  const float* k_scale;
+  const float* v_scale;
+  int64_t num_pages, page_stride, token_stride, head_stride, table_stride;
+  int32_t n_seqs, max_pages, page_size, Hkv, D, type;
+} MxkKvCache;
+
+/* A step's or a prompt's q, k and v into the cache in one pass: per-head RMSNorm (q_norm_w / k_norm_w fp32 [D], NULL
+ * skips it) and rotation of the first `rot` channels of q and k as in mxk_head_norm_rope; q to q_out bf16 [T, H, D],
+ * k and v to the cache (k also to k_out bf16 [T, Hkv, D] unless NULL, which is what mxk_attn_window reads for a
+ * prompt).  Row t is token positions[t] of sequence seq_ids[t] (seq_ids NULL: sequence t); a row with a negative
+ * sequence number is a padding row and nothing is written for it.  Its cos / sin are row rope_rows[t] (NULL:
+ * positions[t]) of the tables fp32 [table_rows, rot / 2].  q, k, v: bf16, head h of row t at t * stride + h * D.
+ * D a multiple of 8 (16 for e4m3), 8 <= D <= 128, strides multiples of 8, q, k, v and outputs 16-byte aligned; rot
+ * even and <= D.  Rows of one call name different (sequence, position) pairs; outputs overlap no input. */
+typedef struct MxkAppendArgs {
+  const mxk_bf16* q;
+  const mxk_bf16* k;
+  const mxk_bf16* v;
+  int64_t T, q_stride, k_stride, v_stride;
+  const float* q_norm_w;
+  const float* k_norm_w;
+  const float* cos;
+  const float* sin;
+  int64_t table_rows;
+  const int32_t* positions;
+  const int32_t* seq_ids;
+  const int32_t* rope_rows;
+  mxk_bf16* q_out;
+  mxk_bf16* k_out;
+  int32_t H, rot, mode;
+  float eps;
+} MxkAppendArgs;
+int mxk_qkv_norm_rope_append(const MxkAppendArgs* args_host, const MxkKvCache* cache_host, mxk_stream_t stream);
+
+/* Attention of one new token of every sequence over its cached tokens (its own among them: append first).
+ *   out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j,  head h reads key head h / (H / Hkv),
+ * over the tokens j of sequence b, j < seq_lens[b] (int32, device), that lie in the window: with left >= 0 only
+ * j >= seq_lens[b] - 1 - left and the first tokens j < sinks; left < 0: all.  Cached tokens outside of it are not
+ * read.  q bf16 [n_seqs, H, D] with rows q_stride elements apart; out bf16 [n_seqs, H, D]; lse fp32 [n_seqs, H] or NULL
+ * receives the natural logarithm of the softmax's denominator.  A sequence of length 0 gives out 0 and lse -inf.
+ * The work is split evenly over the GPU along the cached tokens and joined by a second launch through `workspace`
+ * (mxk_attn_decode_workspace_bytes(cache, H) bytes of device memory, 16-byte aligned, no initial value; calls that may
+ * run at the same time, two captured graphs among them, need one each).  H a multiple of Hkv; D a multiple of 8 (16
+ * for e4m3), at most 128. */
+typedef struct MxkDecodeArgs {
+  const mxk_bf16* q;
+  int64_t q_stride;
+  const int32_t* seq_lens;
+  mxk_bf16* out;
+  float* lse;
+  void* workspace;
+  int64_t left, sinks;
+  int32_t H;
+  float scale;
+} MxkDecodeArgs;
+int64_t mxk_attn_decode_workspace_bytes(const MxkKvCache* cache_host, int H);
+int mxk_attn_decode_paged(const MxkDecodeArgs* args_host, const MxkKvCache* cache_host, mxk_stream_t stream);
+
+/* Attention of a packed batch of sequences.  Sequence b owns rows [cu_q[b], cu_q[b + 1]) of q and out and rows
+ * [cu_k[b], cu_k[b + 1]) of k and v (int32 [n_seqs + 1], device, not decreasing; cu_q NULL: one sequence of all q_rows,
+ * k_rows rows).  Row i of a sequence of Lq rows and Lk keys stands at position p = i + Lk - Lq (the last row at the
+ * last key, so that Lq < Lk continues a prefix) and sees the keys 0 <= j < Lk with
+ *   j <= p + right            (right < 0: no bound; right = 0 is causal)
+ *   j >= p - left or j < sinks  (left < 0: no bound)
+ * out[i, h] = sum_j softmax_j(scale * q[i, h] . k_j) v_j; lse fp32 [q_rows, H] or NULL as above.  A row that sees
+ * nothing gives out 0 and lse -inf; rows of q and out that belong to no sequence are left as they were, and k / v rows
+ * that belong to no sequence, or lie outside of every row's view, do not reach any output whatever they hold.
+ * q, k, v, out: bf16, head h of a row at row * stride + h * D; strides multiples of 8, pointers 16-byte aligned;
+ * head h reads key head h / (H / Hkv); D a multiple of 8, at most 128.  out overlaps no input. */
+typedef struct MxkAttnArgs {
+  const mxk_bf16* q;
+  const mxk_bf16* k;
+  const mxk_bf16* v;
+  mxk_bf16* out;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t q_rows, k_rows, q_stride, k_stride, v_stride, out_stride;
+  int64_t left, right, sinks;
+  int32_t n_seqs, H, Hkv, D;
+  float scale;
+} MxkAttnArgs;
+int mxk_attn_window(const MxkAttnArgs* args_host, mxk_stream_t stream);
+
 /* ---- RoPE tables and timestep embeddings ------------------------------------------------
  * The reference builds these on the host with libm and uploads them once per generation
  * (src/models/qwen_image/dit.cpp:151-185, src/models/minimax_h3/dit.cpp:254-262).  libm's

@@ -47,6 +47,38 @@ class BlockArgs(C.Structure):
     ]
 
 
+class KvCacheArgs(C.Structure):
+    """MxkKvCache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int64), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32),
+                ("Hkv", C.c_int32), ("D", C.c_int32), ("type", C.c_int32)]
+
+
+class AppendArgs(C.Structure):
+    """MxkAppendArgs."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("T", C.c_int64), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p),
+                ("cos", C.c_void_p), ("sin", C.c_void_p), ("table_rows", C.c_int64), ("positions", C.c_void_p),
+                ("seq_ids", C.c_void_p), ("rope_rows", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("H", C.c_int32), ("rot", C.c_int32), ("mode", C.c_int32), ("eps", C.c_float)]
+
+
+class DecodeArgs(C.Structure):
+    """MxkDecodeArgs."""
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("seq_lens", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("workspace", C.c_void_p), ("left", C.c_int64), ("sinks", C.c_int64), ("H", C.c_int32), ("scale", C.c_float)]
+
+
+class AttnArgs(C.Structure):
+    """MxkAttnArgs."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("out_stride", C.c_int64), ("left", C.c_int64),
+                ("right", C.c_int64), ("sinks", C.c_int64), ("n_seqs", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32),
+                ("D", C.c_int32), ("scale", C.c_float)]
+
+
 _P, _I64, _I, _F = C.c_void_p, C.c_int64, C.c_int, C.c_float
 
 # name -> (restype, argtypes); must list every function include/mxk.h declares.
@@ -108,6 +140,10 @@ PROTOTYPES = {
     "mxk_linear_silu_mul": (_I, [_P, _P, _P, _I64, _I64, _I64, _P, _P]),
     "mxk_linear_qkv_norm_rope": (_I, [_P, _P, _P, _I64, _I64, _I, _I, C.POINTER(HeadTensor), _I, _F, _P, _P, _P]),
     "mxk_linear_gated_residual": (_I, [_P, _P, _P, _I64, _I64, _I64, _P, RowMod, _I, _P]),
+    "mxk_qkv_norm_rope_append": (_I, [C.POINTER(AppendArgs), C.POINTER(KvCacheArgs), _P]),
+    "mxk_attn_decode_workspace_bytes": (_I64, [C.POINTER(KvCacheArgs), _I]),
+    "mxk_attn_decode_paged": (_I, [C.POINTER(DecodeArgs), C.POINTER(KvCacheArgs), _P]),
+    "mxk_attn_window": (_I, [C.POINTER(AttnArgs), _P]),
     "mxk_rope_table_expand": (_I, [_P, _P, C.POINTER(C.c_int64), C.POINTER(C.c_int32), C.POINTER(C.c_int32), _I,
                                    C.POINTER(RopeRun), _I, _I64, _I, _P, _P, _P]),
     "mxk_msrope_inv_freq_host": (_I, [C.POINTER(C.c_int32), _I, _F, _P]),

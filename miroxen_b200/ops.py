@@ -13,10 +13,12 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import BlockArgs, HeadTensor, RopeRun, RowMod, check, lib
+from ._lib import (AppendArgs, AttnArgs, BlockArgs, DecodeArgs, HeadTensor, KvCacheArgs, MxkError, RopeRun, RowMod, check,
+                   lib)
 
 ROPE_NONE, ROPE_INTERLEAVED, ROPE_HALF = 0, 1, 2
 ACT_GELU_TANH, ACT_SILU_MUL, ACT_GELU_ERF = 0, 1, 2
+KV_BF16, KV_E4M3 = 0, 1
 Q_MXFP8, Q_NVFP4 = 1, 2  # QMode of src/kernels/blockscale.h:14 (0 = None is not a quantised mode)
 
 __all__ = [
@@ -30,6 +32,7 @@ __all__ = [
     "qwen_latent_encode", "qwen_latent_decode", "h3_latent_video", "h3_latent_audio",
     "bias_gelu_tanh_inplace", "bias_silu_mul", "gated_residual_bias",
     "linear_bf16", "linear_act", "linear_silu_mul", "linear_gated_residual", "linear_qkv_norm_rope", "quantize_nvfp4_known_amax", "layernorm_mod_amax", "rmsnorm_mod_amax", "gated_residual_norm_amax", "act_amax",
+    "KvCache", "qkv_norm_rope_append", "attn_decode_workspace", "attn_decode_paged", "attn_window",
     "norm_path_probe", "NORM_PATH_GENERIC", "NORM_PATH_VECTOR", "NORM_PATH_BULK",
 ]
 
@@ -327,6 +330,75 @@ def linear_qkv_norm_rope(A, W, bias, M, K, H, D, tensors: Sequence[HeadSpec], ep
     """The QKV projection with per-head RMSNorm + rotary embedding in its epilogue (specs: norm_w, out, rot, mode)."""
     arr = (HeadTensor * len(tensors))(*[HeadTensor(None, 0, 0, _p(t.norm_w), _p(t.out), t.rot, t.mode) for t in tensors])
     check(lib().mxk_linear_qkv_norm_rope(_p(A), _p(W), _p(bias), M, K, H, D, arr, len(tensors), eps, _p(cos), _p(sin), _stream(stream)))
+
+
+# ---- paged key/value cache and attention (include/mxk.h: MxkKvCache) ---------------------------
+
+class KvCache:
+    """A paged key/value cache: `k` and `v` [num_pages, page_size, Hkv, D], bf16 or float8_e4m3fn, of any (equal) strides
+    with the channels adjacent - pages with the head outermost are `t.transpose(1, 2)` of a [num_pages, Hkv, page_size, D]
+    tensor - `page_table` int32 [n_seqs, max_pages]; `k_scale`, `v_scale` fp32 [Hkv] of an e4m3 cache (None: 1).  Keeps
+    the tensors alive; what they hold may change between calls, their addresses and shapes may not."""
+
+    def __init__(self, k, v, page_table, k_scale=None, v_scale=None):
+        if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or v.dtype != k.dtype:
+            raise MxkError(f"KvCache: k and v must both be bfloat16 or float8_e4m3fn (got {k.dtype}, {v.dtype})")
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1:
+            raise MxkError("KvCache: k and v must be [num_pages, page_size, Hkv, D] of equal strides, channels adjacent")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise MxkError("KvCache: page_table must be int32 [n_seqs, max_pages], pages of a sequence adjacent")
+        for s in (k_scale, v_scale):
+            if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (k.shape[2],) or not s.is_contiguous()):
+                raise MxkError("KvCache: k_scale and v_scale must be contiguous float32 [Hkv]")
+            if s is not None and k.dtype == torch.bfloat16:
+                raise MxkError("KvCache: scales belong to an e4m3 cache")
+        if any(t is not None and t.device != k.device for t in (v, page_table, k_scale, v_scale)):
+            raise MxkError("KvCache: all tensors must be on one device")
+        self.k, self.v, self.page_table, self.k_scale, self.v_scale = k, v, page_table, k_scale, v_scale
+        self._args = KvCacheArgs(_p(k), _p(v), _p(page_table), _p(k_scale), _p(v_scale), k.shape[0], k.stride(0), k.stride(1),
+                                 k.stride(2), page_table.stride(0), page_table.shape[0], page_table.shape[1], k.shape[1],
+                                 k.shape[2], k.shape[3], KV_BF16 if k.dtype == torch.bfloat16 else KV_E4M3)
+
+
+def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, table_rows, rot, mode, cache: KvCache, positions,
+                         q_out, seq_ids=None, rope_rows=None, k_out=None, q_stride=None, k_stride=None, v_stride=None, stream=None):
+    """Per-head norm and rotation of q and k, q to q_out, k and v into the cache's pages (k also to k_out), in one pass."""
+    c = cache._args
+    if D != c.D:
+        raise MxkError(f"qkv_norm_rope_append: D={D} and a cache of D={c.D}")
+    kv = c.Hkv * D
+    a = AppendArgs(_p(q), _p(k), _p(v), T, H * D if q_stride is None else q_stride, kv if k_stride is None else k_stride,
+                   kv if v_stride is None else v_stride, _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), table_rows, _p(positions),
+                   _p(seq_ids), _p(rope_rows), _p(q_out), _p(k_out), H, rot, mode, eps)
+    check(lib().mxk_qkv_norm_rope_append(a, c, _stream(stream)))
+
+
+def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
+    """Scratch memory for attn_decode_paged with this cache and head count: keep one for each stream or graph that may
+    run at the same time as another."""
+    n = lib().mxk_attn_decode_workspace_bytes(cache._args, H)
+    if n < 0:
+        check(n)
+    return torch.empty(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def attn_decode_paged(q, cache: KvCache, seq_lens, H, scale, out, left=-1, sinks=0, q_stride=None, lse=None, *, workspace, stream=None):
+    """Attention of one new token of every sequence over its tokens in the cache."""
+    c = cache._args
+    a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), left, sinks, H, scale)
+    check(lib().mxk_attn_decode_paged(a, c, _stream(stream)))
+
+
+def attn_window(q, k, v, q_rows, k_rows, H, Hkv, D, scale, out, left=-1, right=-1, sinks=0, cu_q=None, cu_k=None, n_seqs=None,
+                q_stride=None, k_stride=None, v_stride=None, out_stride=None, lse=None, stream=None):
+    """Attention of a packed batch of sequences (cu_q, cu_k: int32 [n_seqs + 1] first rows; None: one sequence) with a
+    window of `left` / `right` keys (-1: no bound; right = 0: causal) and `sinks` first keys that stay visible."""
+    if n_seqs is None:
+        n_seqs = 1 if cu_q is None else cu_q.numel() - 1
+    a = AttnArgs(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k), q_rows, k_rows, H * D if q_stride is None else q_stride,
+                 Hkv * D if k_stride is None else k_stride, Hkv * D if v_stride is None else v_stride,
+                 H * D if out_stride is None else out_stride, left, right, sinks, n_seqs, H, Hkv, D, scale)
+    check(lib().mxk_attn_window(a, _stream(stream)))
 
 
 def _qmat_for(x, rows, dim, out):
