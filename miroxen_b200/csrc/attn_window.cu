@@ -5,6 +5,28 @@
 //
 // Row i of a sequence of Lq rows and Lk keys stands at p = i + Lk - Lq and sees j <= p + right (right >= 0) that are
 // j >= p - left (left >= 0) or j < sinks.
+//
+// Two matrix products of 4 D flops per pair with one exponential between: the tensor cores bound it, the exponentials
+// (16 per clock and SM) nearly as much.  One CTA of 384 threads holds 256 rows of one head as two halves of 128:
+//   warps 0-3, 4-7: the softmax of one half each, a thread per row.  A score tile (128 rows x 128 keys, fp32) comes from
+//                   tensor memory into registers, its row maximum, exponentials and their sum are taken there, and the
+//                   probabilities go back as bf16 (the type of V, which the product needs) over the scores they came from;
+//   warp 8:         issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory.  While one half's
+//                   softmax runs, the other half's products do;
+//   warp 9:         TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
+//   warps 10, 11:   only complete the group of four whose registers the softmax warps take over (setmaxnreg).
+// Tensor memory: S (with P in it) and O of both halves, 4 x 128 columns.  The running maximum that the exponentials use
+// moves only when it would grow by more than 2^8 (results are the same: every sum is relative to it), so O is rescaled
+// rarely, by the half's own warps, which at that point know that no product is under way on it.
+// Blocks of 128 keys outside of every row's view are not visited; only blocks at the edge of some row's view pay for the
+// mask.  There, what lies out of view must not reach 0 * v: value rows behind the sequence are zeroed in shared memory, and
+// if any other value of the block is not finite the rows are taken again by a plain loop (row_attention) that never touches
+// what a row does not see.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "bulk_copy.cuh"
 #include "common.cuh"
 #include "kv_cache.cuh"
 
@@ -108,35 +130,472 @@ __device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k
   if (lane == 0 && a.lse) a.lse[row * a.H + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-__global__ void __launch_bounds__(256) attn_rows_kernel(const __grid_constant__ AttnLaunch L) {
-  __shared__ float qs[8][MXK_ATTN_MAX_HEAD_DIM];
+// ---- tensor-core kernel ----------------------------------------------------------------------------------------
+
+constexpr int kM = 128, kN = 128;              // rows of a half, keys of a block
+constexpr int kMmaWarp = 8, kTmaWarp = 9, kThreadsW = 384;
+constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channel tile
+// Registers a thread: 384 x 168 at launch; a softmax thread holds a row of 128 scores, the warps of the third group need few.
+constexpr int kRegsSoft = 208, kRegsOther = 88;
+static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
+constexpr unsigned kTmemS = 0, kTmemO = 256, kTmemCols = 512;
+constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
+
+template <int DP>
+struct WindowCfg {
+  static constexpr int kSubs = DP / 64;               // 64-channel tiles of a row
+  static constexpr int kTileBytes = kSubs * kSub;     // Q half, K block, V block
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+};
+
+template <int DP>
+struct __align__(1024) WindowSmem {
+  unsigned char q[2][WindowCfg<DP>::kTileBytes];
+  unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
+  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], p_full[2], o_full[2];
+  unsigned tmem_base;
+  int poison[2];  // a value that is not finite lies in a block at the edge of the half's view
+  int scan[kThreadsW / 32], found[4];
+};
+
+__device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+               "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive1(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit_to(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (+)= A B, A and B from shared memory
+__device__ __forceinline__ void mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(idesc), "r"(acc)
+               : "memory");
+}
+// D (+)= A B, A from tensor memory
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, unsigned acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(idesc), "r"(acc)
+               : "memory");
+}
+// Shared-memory matrix descriptors under the 128-byte swizzle (1024-byte aligned tiles of 128-byte rows): start address,
+// leading and stride offsets in 16-byte units, version 1, layout type 2.
+//   Q, K: K-major (a row's channels are adjacent): eight rows every 1024 bytes (stride offset).
+//   V: MN-major (the keys are the contraction, the channels adjacent): eight keys every 1024 bytes (stride offset), the next
+//      64 channels one 16 KB tile further (leading offset).
+__device__ __forceinline__ uint64_t desc_sw128(unsigned addr, unsigned leading) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(leading >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// kind::f16, fp32 accumulator, bf16 operands; b_mn: B is MN-major
+template <int M, int N, bool B_MN>
+constexpr unsigned kInstr = (1u << 4) | (1u << 7) | (1u << 10) | (unsigned(B_MN) << 16) | (unsigned(N >> 3) << 17) | (unsigned(M >> 4) << 24);
+#define MXK_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
+#define MXK_R32(a, i) \
+  MXK_R4(a, i), MXK_R4(a, i + 4), MXK_R4(a, i + 8), MXK_R4(a, i + 12), MXK_R4(a, i + 16), MXK_R4(a, i + 20), MXK_R4(a, i + 24), MXK_R4(a, i + 28)
+// 32 columns of this thread's lane; tmem_wait_ld() before the first use
+__device__ __forceinline__ void tmem_ld32(unsigned addr, unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : MXK_R32(r, 0)
+      : "r"(addr)
+      : "memory");
+}
+// The loads have landed; the empty statements tie the registers to this point.
+__device__ __forceinline__ void tmem_wait_ld(unsigned (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_touch(unsigned (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_st32(unsigned addr, const unsigned (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+struct WindowLaunch {
+  AttnLaunch L;
+  int halves;     // 128-row halves of a tile: 2, or 1 where that leaves SMs idle
+  int max_tiles;  // the grid has max_tiles * H CTAs
+};
+
+// What a CTA works on: rows [r0, r0 + rows) of a sequence that starts at row q0 / key k0 and has nq rows, nk keys.
+struct WindowTile {
+  int q0, nq, k0, nk, r0, rows;
+};
+
+// Tile `want` counted over the sequences, with the whole CTA; rows = 0: there is none.
+__device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int want, int* scan, int* found) {
+  const MxkAttnArgs& a = W.L.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tile_rows = kM * W.halves;
+  WindowTile t{0, int(a.q_rows), 0, int(a.k_rows), 0, 0};
+  if (!a.cu_q) {
+    t.r0 = want * tile_rows;
+    t.rows = min(tile_rows, t.nq - t.r0);
+    return t;
+  }
+  // thread t counts a contiguous share of the sequences
+  const int n = a.n_seqs, share = (n + kThreadsW - 1) / kThreadsW, b0 = min(n, tid * share), b1 = min(n, b0 + share);
+  auto tiles = [&](int b) {
+    const int q0 = cu_at(a.cu_q, b, a.q_rows, 0, W.L.err);
+    return (cu_at(a.cu_q, b + 1, a.q_rows, q0, W.L.err) - q0 + tile_rows - 1) / tile_rows;
+  };
+  int mine = 0;
+  for (int b = b0; b < b1; b++) mine += tiles(b);
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) scan[warp] = incl;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  int at = incl - mine;
+  for (int w = 0; w < warp; w++) at += scan[w];
+  if (want >= at && want < at + mine) {
+    int b = b0;
+    for (int k = tiles(b); want >= at + k; k = tiles(b)) at += k, b++;
+    found[0] = b, found[1] = want - at;
+  }
+  __syncthreads();
+  const int b = found[0];
+  if (b < 0) return t;
+  t.q0 = cu_at(a.cu_q, b, a.q_rows, 0, W.L.err), t.nq = cu_at(a.cu_q, b + 1, a.q_rows, t.q0, W.L.err) - t.q0;
+  t.k0 = cu_at(a.cu_k, b, a.k_rows, 0, W.L.err), t.nk = cu_at(a.cu_k, b + 1, a.k_rows, t.k0, W.L.err) - t.k0;
+  t.r0 = found[1] * tile_rows;
+  t.rows = min(tile_rows, t.nq - t.r0);
+  return t;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreadsW, 1)
+    window_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const __grid_constant__ WindowLaunch W) {
+  using Cfg = WindowCfg<DP>;
+  constexpr int kSt = Cfg::kStages;
+  extern __shared__ unsigned char smem_raw[];
+  WindowSmem<DP>& sm = *reinterpret_cast<WindowSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const AttnLaunch& L = W.L;
   const MxkAttnArgs& a = L.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the tiles at the end of a causal sequence have the most keys: they start first
+  const int head = int(blockIdx.x) % a.H, want = W.max_tiles - 1 - int(blockIdx.x) / a.H, kv_head = head / L.group;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.o_full[i]), 1);
+      mbar_init(smem_u32(&sm.p_full[i]), 4);
+      sm.poison[i] = 0;
+    }
+    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5;
-  const int64_t row = int64_t(blockIdx.x) * 8 + warp;
-  if (a.cu_q && blockIdx.x == 0 && blockIdx.y == 0)  // every end, those that no row looks at too
-    for (int b = threadIdx.x; b < a.n_seqs; b += blockDim.x) {
-      cu_at(a.cu_q, b + 1, a.q_rows, cu_at(a.cu_q, b, a.q_rows, 0, L.err), L.err);
-      cu_at(a.cu_k, b + 1, a.k_rows, cu_at(a.cu_k, b, a.k_rows, 0, L.err), L.err);
-    }
-  if (row >= a.q_rows) return;
-  int q0 = 0, q1 = int(a.q_rows), k0 = 0, k1 = int(a.k_rows);
-  if (a.cu_q) {
-    // the sequence that the row lies in: the first whose end lies behind it
-    int b = 0, lo = 0, hi = a.n_seqs;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.cu_q[mid + 1] > row) hi = mid;
-      else lo = mid + 1;
-    }
-    b = lo;
-    if (b >= a.n_seqs || a.cu_q[b] > row) return;  // a row of no sequence
-    q0 = cu_at(a.cu_q, b, a.q_rows, 0, L.err), q1 = cu_at(a.cu_q, b + 1, a.q_rows, q0, L.err);
-    k0 = cu_at(a.cu_k, b, a.k_rows, 0, L.err), k1 = cu_at(a.cu_k, b + 1, a.k_rows, k0, L.err);
+  const WindowTile t = find_tile(W, want, sm.scan, sm.found);
+  if (t.rows <= 0) return;  // the whole CTA
+  const int halves = t.rows > kM ? 2 : 1;
+
+  // blocks of keys that some row of the tile sees: n_sink from the front, the others from block wb0 on
+  const int64_t shift = int64_t(t.nk) - t.nq;  // a row's position is its number + shift
+  const Seen s_first = seen_by(a, t.r0 + shift, t.nk), s_last = seen_by(a, t.r0 + t.rows - 1 + shift, t.nk);
+  const int wb0 = s_first.lo / kN, wb1 = s_last.hi > s_first.lo ? (s_last.hi + kN - 1) / kN : wb0;
+  const int n_sink = min((s_last.first + kN - 1) / kN, wb0);
+  const int n_blocks = n_sink + wb1 - wb0;
+  auto block_at = [&](int j) { return j < n_sink ? j : wb0 + j - n_sink; };
+
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const int nk = k1 - k0;
-  row_attention(L, row, int(blockIdx.y), k0, row - q0 + nk - (q1 - q0), nk, qs[warp]);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const unsigned tmem = sm.tmem_base;
+
+  bool ok = true;
+  int issued = 0;  // TMA lane: stage fills issued so far
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kTmaWarp && lane == 0 && n_blocks > 0) {
+      for (int h = 0; h < halves; h++) {
+        const unsigned bar = smem_u32(&sm.q_full[h]);
+        mbar_expect_tx(bar, Cfg::kTileBytes);
+        for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.q[h]) + c * kSub, &map_q, c * 64, head, t.q0 + t.r0 + h * kM, bar);
+      }
+      // fill 2 j: K of block j; fill 2 j + 1: its V
+      for (issued = 0; issued < 2 * n_blocks; issued++) {
+        const int st = issued % kSt;
+        if (issued >= kSt && !mbar_wait(smem_u32(&sm.empty[st]), unsigned(issued / kSt - 1) & 1u)) {
+          ok = false;
+          break;
+        }
+        const unsigned bar = smem_u32(&sm.full[st]);
+        mbar_expect_tx(bar, Cfg::kTileBytes);
+        const int key = t.k0 + block_at(issued >> 1) * kN;
+        const CUtensorMap* map = (issued & 1) ? &map_v : &map_k;
+        for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.kv[st]) + c * kSub, map, c * 64, kv_head, key, bar);
+      }
+    } else if (warp == kMmaWarp && lane == 0 && n_blocks > 0) {
+      constexpr unsigned id_qk = kInstr<kM, kN, false>, id_pv = kInstr<kM, DP, true>;
+      auto scores = [&](int h, int fill) {  // S of half h from the K tile of this fill
+        const unsigned qa = smem_u32(sm.q[h]), ka = smem_u32(sm.kv[fill % kSt]);
+#pragma unroll
+        for (int c = 0; c < Cfg::kSubs; c++)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            mma_ss(tmem + kTmemS + unsigned(h) * 128, desc_sw128(qa + c * kSub, 16) + uint64_t(2 * k), desc_sw128(ka + c * kSub, 16) + uint64_t(2 * k), id_qk,
+                   (c | k) != 0 ? 1u : 0u);
+        commit_to(smem_u32(&sm.s_full[h]));
+      };
+      auto wait_fill = [&](int fill) {
+        const bool r = mbar_wait(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u);
+        fence_after();
+        return r;
+      };
+      ok = wait_fill(0);
+      for (int h = 0; h < halves && ok; h++) {
+        ok = mbar_wait(smem_u32(&sm.q_full[h]), 0);
+        if (ok) scores(h, 0);
+      }
+      if (ok) commit_to(smem_u32(&sm.empty[0]));
+      for (int j = 0; j < n_blocks && ok; j++) {
+        const int fv = 2 * j + 1, fk = 2 * j + 2;
+        if (!(ok = wait_fill(fv))) break;
+        for (int h = 0; h < halves; h++) {
+          if (!(ok = mbar_wait(smem_u32(&sm.p_full[h]), unsigned(j) & 1u))) break;
+          fence_after();
+          const unsigned va = smem_u32(sm.kv[fv % kSt]);
+#pragma unroll
+          for (int k = 0; k < kN / 16; k++)  // 16 keys: 8 columns of P, 2048 bytes of V
+            mma_ts(tmem + kTmemO + unsigned(h) * 128, tmem + kTmemS + unsigned(h) * 128 + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128), id_pv,
+                   (j | k) != 0 ? 1u : 0u);
+          if (h == halves - 1) commit_to(smem_u32(&sm.empty[fv % kSt]));
+          if (j + 1 < n_blocks) {
+            if (h == 0 && !(ok = wait_fill(fk))) break;
+            scores(h, fk);
+            if (h == halves - 1) commit_to(smem_u32(&sm.empty[fk % kSt]));
+          } else {
+            commit_to(smem_u32(&sm.o_full[h]));
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+    if ((warp >> 2) < halves) {
+      // ---- softmax of half h: thread (warp & 3) * 32 + lane owns that row ----
+      const int h = warp >> 2, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
+      const int rows_h = min(kM, t.rows - h * kM);
+      const unsigned lanes = unsigned((warp & 3) * 32) << 16;
+      const unsigned ts = tmem + lanes + kTmemS + unsigned(h) * 128, to = tmem + lanes + kTmemO + unsigned(h) * 128;
+      const Seen mine = seen_by(a, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
+      // the first row of the half has the nearest end, the last row the farthest window start
+      const Seen h_first = seen_by(a, rh0 + shift, t.nk), h_last = seen_by(a, rh0 + rows_h - 1 + shift, t.nk);
+      float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), sum
+      for (int j = 0; j < n_blocks; j++) {
+        const int key0 = block_at(j) * kN;
+        const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
+        if (!(ok = mbar_wait(smem_u32(&sm.s_full[h]), unsigned(j) & 1u))) break;
+        fence_after();
+        unsigned s[4][32];
+  #pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, s[c]);
+        tmem_wait_ld(s[0]);
+        tmem_touch(s[1]), tmem_touch(s[2]), tmem_touch(s[3]);
+        if (edge) {
+          const int first = mine.first - key0, lo = mine.lo - key0, hi = mine.hi - key0;
+  #pragma unroll
+          for (int c = 0; c < 4; c++)
+  #pragma unroll
+            for (int i = 0; i < 32; i++) {
+              const int k = 32 * c + i;
+              if (!(k < first || (k >= lo && k < hi))) s[c][i] = 0xff800000u;
+            }
+          // V of this block: zero what lies behind the sequence, look for values that are not finite in the rest
+          const int fv = 2 * j + 1;
+          if (!(ok = mbar_wait(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u))) break;
+          uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
+          const int there = t.nk - key0;
+          bool bad = false;
+  #pragma unroll 4
+          for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM) {
+            if (((i >> 3) & 127) < there) {
+              const uint4 x = vt[i];
+              constexpr unsigned e = 0x7f807f80u;
+              bad |= (__vcmpeq2(x.x & e, e) | __vcmpeq2(x.y & e, e) | __vcmpeq2(x.z & e, e) | __vcmpeq2(x.w & e, e)) != 0;
+            } else {
+              vt[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          if (bad) sm.poison[h] = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        float mx = -INFINITY;
+  #pragma unroll
+        for (int c = 0; c < 4; c++)
+  #pragma unroll
+          for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[c][i]));
+        const bool grow = (mx - m) * L.scale2 > kSlack;  // also the first finite score (m = -inf); false for NaN
+        if (__any_sync(0xffffffffu, grow)) {
+          float f = 1.f;
+          if (grow) {
+            f = ex2_approx((m - mx) * L.scale2);
+            m = mx, l *= f;
+          }
+          if (j > 0) {  // every product issued so far has retired: s_full of this block was signalled behind them
+  #pragma unroll
+            for (int c = 0; c < DP / 32; c++) {
+              unsigned o[32];
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait_ld(o);
+  #pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(to + 32 * c, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m * L.scale2;
+  #pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned p[16];
+  #pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i]), L.scale2, -base));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), L.scale2, -base));
+            l += p0 + p1;
+            p[i] = pack_bf16(p0, p1);
+          }
+          tmem_st16(ts + 16 * c, p);
+        }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(smem_u32(&sm.p_full[h]));
+      }
+      // ---- output ----
+      if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(&sm.o_full[h]), 0);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        fence_after();
+        const int64_t row = int64_t(t.q0) + rh0 + row_h;
+        const bool on = row_h < rows_h;
+        if (n_blocks > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
+          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 3) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
+          for (int r = (warp & 3) * 32; r < min((warp & 3) * 32 + 32, rows_h); r++)
+            row_attention(L, int64_t(t.q0) + rh0 + r, head, t.k0, rh0 + r + shift, t.nk, qs);
+        } else {
+          const bool some = l > 0.f || l != l;
+          const float f = some ? 1.f / l : 0.f;
+          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D;
+  #pragma unroll 1
+          for (int c = 0; c < DP / 32; c++) {
+            unsigned o[32];
+            if (n_blocks > 0) {
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait_ld(o);
+            }
+            if (!on) continue;
+  #pragma unroll
+            for (int i = 0; i < 4; i++) {
+              float v[8];
+  #pragma unroll
+              for (int e = 0; e < 8; e++) v[e] = some ? __uint_as_float(o[8 * i + e]) * f : 0.f;
+              if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
+            }
+          }
+          if (on && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
+        }
+      }
+    }
+  }
+
+  if (!ok && L.err) atomicExch(L.err, kErrBulkTimeout);
+  fence_before();
+  // Every role's waits are bounded, so all threads arrive here.  After a failure the copies under way get a bounded chance
+  // to land before the shared memory goes.
+  if (__syncthreads_or(!ok) != 0) {
+    if (tid == kTmaWarp * 32) {
+      for (int h = 0; h < halves; h++) mbar_wait(smem_u32(&sm.q_full[h]), 0);
+      for (int i = issued > kSt ? issued - kSt : 0; i < issued; i++) mbar_wait(smem_u32(&sm.full[i % kSt]), unsigned(i / kSt) & 1u);
+    }
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static std::atomic<EncodeFn> cached{nullptr};
+  EncodeFn f = cached.load(std::memory_order_acquire);
+  if (f) return f;
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess || !p) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  f = reinterpret_cast<EncodeFn>(p);
+  cached.store(f, std::memory_order_release);
+  return f;
+}
+
+// bf16 [rows, heads, D]: boxes of 64 channels of one head of 128 rows, 128-byte swizzle; what lies outside reads as 0.
+int make_map(const char* name, CUtensorMap* map, const void* base, int64_t rows, int heads, int D, int64_t stride) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return fail(MXK_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", name);
+  if (rows == 1) stride = int64_t(heads) * D;  // never used
+  const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(rows)};
+  const cuuint64_t strides[2] = {cuuint64_t(D) * 2, cuuint64_t(stride) * 2};
+  const cuuint32_t box[3] = {64, 1, 128};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MXK_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with code %d", name, int(r));
+  return MXK_OK;
+}
+
+template <int DP>
+int launch_window(const char* name, WindowLaunch& W, cudaStream_t s) {
+  const MxkAttnArgs& a = W.L.a;
+  CUtensorMap mq, mk, mv;
+  if (int rc = make_map(name, &mq, a.q, a.q_rows, a.H, a.D, a.q_stride)) return rc;
+  // without a key nothing is loaded; the maps then only have to be valid
+  if (int rc = make_map(name, &mk, a.k_rows > 0 ? a.k : a.q, a.k_rows > 0 ? a.k_rows : 1, a.k_rows > 0 ? a.Hkv : 1, a.D, a.k_stride)) return rc;
+  if (int rc = make_map(name, &mv, a.k_rows > 0 ? a.v : a.q, a.k_rows > 0 ? a.k_rows : 1, a.k_rows > 0 ? a.Hkv : 1, a.D, a.v_stride)) return rc;
+  auto k = window_kernel<DP>;
+  const size_t smem = sizeof(WindowSmem<DP>) + 1024;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return fail(MXK_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(e));
+  const int64_t ctas = int64_t(W.max_tiles) * a.H;
+  if (ctas >= (int64_t(1) << 31)) return fail(MXK_ERR_TOO_LARGE, "%s: %lld tiles", name, (long long)ctas);
+  launch_pdl(k, dim3(unsigned(ctas)), dim3(kThreadsW), smem, s, mq, mk, mv, W);
+  return after_launch(name);
 }
 
 }  // namespace
@@ -173,6 +632,15 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   L.group = a.H / a.Hkv;
   L.scale2 = a.scale * kLog2e;
   L.err = device_error_word();
-  launch_pdl(attn_rows_kernel, dim3(unsigned(ceil_div(a.q_rows, 8)), unsigned(a.H)), dim3(256), 0, as_stream(stream), L);
-  return after_launch(name);
+  // bounds that no position reaches
+  if (L.a.left >= (int64_t(1) << 32)) L.a.left = -1;
+  if (L.a.right >= (int64_t(1) << 32)) L.a.right = -1;
+  WindowLaunch W{L, 2, 0};
+  // at most one tile per sequence is not full
+  auto tiles = [&](int rows) { return a.n_seqs == 1 ? ceil_div(a.q_rows, rows) : a.q_rows / rows + (a.n_seqs < a.q_rows ? a.n_seqs : a.q_rows); };
+  if (tiles(2 * kM) * a.H <= sm_count() / 2) W.halves = 1;  // twice the CTAs still fit the GPU at once
+  const int64_t most = tiles(W.halves * kM);
+  if (most >= (int64_t(1) << 31)) return fail(MXK_ERR_TOO_LARGE, "%s: %lld tiles", name, (long long)most);
+  W.max_tiles = int(most);
+  return a.D <= 64 ? launch_window<64>(name, W, as_stream(stream)) : launch_window<128>(name, W, as_stream(stream));
 }
