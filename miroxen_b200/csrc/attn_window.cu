@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       // fill 2 j: K of block j; fill 2 j + 1: its V
       for (issued = 0; issued < 2 * n_blocks; issued++) {
         const int st = issued % kSt;
-        if (issued >= kSt && !mbar_wait(smem_u32(&sm.empty[st]), unsigned(issued / kSt - 1) & 1u)) {
+        if (issued >= kSt && !mbar_wait_spin(smem_u32(&sm.empty[st]), unsigned(issued / kSt - 1) & 1u)) {
           ok = false;
           break;
         }
@@ -369,13 +369,13 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         commit_to(smem_u32(&sm.s_full[h]));
       };
       auto wait_fill = [&](int fill) {
-        const bool r = mbar_wait(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u);
+        const bool r = mbar_wait_spin(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u);
         fence_after();
         return r;
       };
       ok = wait_fill(0);
       for (int h = 0; h < halves && ok; h++) {
-        ok = mbar_wait(smem_u32(&sm.q_full[h]), 0);
+        ok = mbar_wait_spin(smem_u32(&sm.q_full[h]), 0);
         if (ok) scores(h, 0);
       }
       if (ok) commit_to(smem_u32(&sm.empty[0]));
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         const int fv = 2 * j + 1, fk = 2 * j + 2;
         if (!(ok = wait_fill(fv))) break;
         for (int h = 0; h < halves; h++) {
-          if (!(ok = mbar_wait(smem_u32(&sm.p_full[h]), unsigned(j) & 1u))) break;
+          if (!(ok = mbar_wait_spin(smem_u32(&sm.p_full[h]), unsigned(j) & 1u))) break;
           fence_after();
           const unsigned va = smem_u32(sm.kv[fv % kSt]);
 #pragma unroll
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       for (int j = 0; j < n_blocks; j++) {
         const int key0 = block_at(j) * kN;
         const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
-        if (!(ok = mbar_wait(smem_u32(&sm.s_full[h]), unsigned(j) & 1u))) break;
+        if (!(ok = mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(j) & 1u))) break;
         fence_after();
         unsigned s[4][32];
   #pragma unroll
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             }
           // V of this block: zero what lies behind the sequence, look for values that are not finite in the rest
           const int fv = 2 * j + 1;
-          if (!(ok = mbar_wait(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u))) break;
+          if (!(ok = mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u))) break;
           uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
           const int there = t.nk - key0;
           bool bad = false;
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         if (lane == 0) mbar_arrive1(smem_u32(&sm.p_full[h]));
       }
       // ---- output ----
-      if (ok && n_blocks > 0) ok = mbar_wait(smem_u32(&sm.o_full[h]), 0);
+      if (ok && n_blocks > 0) ok = mbar_wait_spin(smem_u32(&sm.o_full[h]), 0);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         fence_after();

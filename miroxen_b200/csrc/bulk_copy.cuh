@@ -47,6 +47,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
   }
   return false;
 }
+// The same without the sleeps, for hand-overs between warps that happen every microsecond or two: there the back-off of
+// mbar_wait would be longer than the wait itself.
+constexpr unsigned kSpinTries = 1u << 18;
+__device__ __forceinline__ bool mbar_wait_spin(unsigned bar, unsigned parity) {
+  for (unsigned i = 0; i < kSpinTries; i++)
+    if (mbar_try(bar, parity)) return true;
+  return false;
+}
 // 1-D bulk copy global -> this CTA's shared memory; src, dst and bytes are multiples of 16.
 __device__ __forceinline__ void bulk_g2s(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
