@@ -139,6 +139,7 @@ constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channe
 constexpr int kRegsSoft = 208, kRegsOther = 88;
 static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
 constexpr unsigned kTmemS = 0, kTmemO = 256, kTmemCols = 512;
+constexpr int kPart = 96;                      // keys after which the first part of the probabilities is handed over
 constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
 
 template <int DP>
@@ -152,7 +153,7 @@ template <int DP>
 struct __align__(1024) WindowSmem {
   unsigned char q[2][WindowCfg<DP>::kTileBytes];
   unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
-  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], p_full[2], o_full[2];
+  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], p_part[2], p_full[2], o_full[2];
   unsigned tmem_base;
   int poison[2];  // a value that is not finite lies in a block at the edge of the half's view
   int scan[kThreadsW / 32], found[4];
@@ -166,20 +167,33 @@ __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map
 __device__ __forceinline__ void mbar_arrive1(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit_to(unsigned bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The matrix instructions are issued by one lane of a converged warp: the whole warp computes the operands (which then are
+// uniform registers, as the instruction wants them) and the instruction itself is predicated.  Issued from a branch of one
+// lane, every operand is moved between register files first, and the issue takes longer than the product.
+__device__ __forceinline__ unsigned elect_lane() {
+  unsigned r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void commit_to(unsigned bar, unsigned leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
+      : "memory");
 }
 // D (+)= A B, A and B from shared memory
-__device__ __forceinline__ void mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-               "l"(b), "r"(idesc), "r"(acc)
-               : "memory");
+__device__ __forceinline__ void mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc, unsigned leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
 }
 // D (+)= A B, A from tensor memory
-__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, unsigned acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-               "l"(b), "r"(idesc), "r"(acc)
-               : "memory");
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, unsigned acc, unsigned leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
 }
 // Shared-memory matrix descriptors under the 128-byte swizzle (1024-byte aligned tiles of 128-byte rows): start address,
 // leading and stride offsets in 16-byte units, version 1, layout type 2.
@@ -214,13 +228,12 @@ __device__ __forceinline__ void tmem_touch(unsigned (&r)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i]));
 }
-__device__ __forceinline__ void tmem_st32(unsigned addr, const unsigned (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(unsigned addr, unsigned (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : MXK_R4(r, 0), MXK_R4(r, 4), MXK_R4(r, 8), MXK_R4(r, 12)
+      : "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]) {
@@ -230,7 +243,75 @@ __device__ __forceinline__ void tmem_st16(unsigned addr, const unsigned (&r)[16]
       "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// This warp's stores to tensor memory so far are for the tensor pipe to read.
+__device__ __forceinline__ void hand_over(unsigned long long* bar, int lane) {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive1(smem_u32(bar));
+}
+
+// Pairs of fp32 operations (one issue slot for two).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^x of a pair on the multiply-add pipe, for -126 <= x < 127: x = n + f, |f| <= 1/2, n by adding and taking away 1.5 * 2^23
+// (the integer then stands in the low bits), 2^f by a polynomial of degree 5 fitted to the least relative error on
+// [-1/2, 1/2] (7.5e-8, below the hardware's 2^x), n added to its exponent.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
+  const uint64_t magic = pair(12582912.f, 12582912.f), unmagic = pair(-12582912.f, -12582912.f), minus = pair(-1.f, -1.f);
+  const uint64_t r = add2(x, magic), n = add2(r, unmagic), f = fma2(n, minus, x);
+  uint64_t p = fma2(f, pair(1.3276472454890609e-3f, 1.3276472454890609e-3f), pair(9.675540961325169e-3f, 9.675540961325169e-3f));
+  p = fma2(p, f, pair(5.550713092088699e-2f, 5.550713092088699e-2f));
+  p = fma2(p, f, pair(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, pair(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, f, pair(1.0000001192092896f, 1.0000001192092896f));
+  float pl, ph, rl, rh;
+  split(p, pl, ph), split(r, rl, rh);
+  lo = __uint_as_float(__float_as_uint(pl) + (__float_as_uint(rl) << 23));
+  hi = __uint_as_float(__float_as_uint(ph) + (__float_as_uint(rh) << 23));
+}
+// Of every eight pairs of scores this many take their 2^x on the multiply-add pipe, the others on the special-function unit.
+#ifndef MXK_POLY
+#define MXK_POLY 0
+#endif
+constexpr int kPolyPairs = MXK_POLY;
+
+// Probabilities of 32 scores: p = 2^(s * scale2 - base), their sum into l2 (two partial sums), rounded to bf16 in pairs.
+template <bool POLY>
+__device__ __forceinline__ void exp_chunk(const unsigned (&s)[32], uint64_t scale2, uint64_t neg_base, uint64_t (&l2)[2], unsigned (&p)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, neg_base);
+    float lo, hi, p0, p1;
+    split(x, lo, hi);
+    if (POLY && (i % 8) * kPolyPairs % 8 + kPolyPairs >= 8) {
+      exp2_pair(pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f)), p0, p1);
+    } else {
+      p0 = ex2_approx(lo), p1 = ex2_approx(hi);
+    }
+    l2[i & 1] = add2(l2[i & 1], pair(p0, p1));
+    p[i] = pack_bf16(p0, p1);
+  }
+}
 
 struct WindowLaunch {
   AttnLaunch L;
@@ -297,14 +378,14 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   WindowSmem<DP>& sm = *reinterpret_cast<WindowSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const AttnLaunch& L = W.L;
   const MxkAttnArgs& a = L.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // the tiles at the end of a causal sequence have the most keys: they start first
   const int head = int(blockIdx.x) % a.H, want = W.max_tiles - 1 - int(blockIdx.x) / a.H, kv_head = head / L.group;
 
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.o_full[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), 4);
+      mbar_init(smem_u32(&sm.p_part[i]), 4), mbar_init(smem_u32(&sm.p_full[i]), 4);
       sm.poison[i] = 0;
     }
     for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
@@ -323,6 +404,19 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   const int n_sink = min((s_last.first + kN - 1) / kN, wb0);
   const int n_blocks = n_sink + wb1 - wb0;
   auto block_at = [&](int j) { return j < n_sink ? j : wb0 + j - n_sink; };
+  // which blocks some row of half h sees: those in front of `sinks`, and [from, last]
+  struct HalfView {
+    int sinks, from, last;
+    __device__ __forceinline__ bool has(int block) const { return block <= last && (block < sinks || block >= from); }
+  } view[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const Seen f = seen_by(a, t.r0 + h * kM + shift, t.nk), e = seen_by(a, t.r0 + min((h + 1) * kM, t.rows) - 1 + shift, t.nk);
+    view[h].from = f.lo / kN;
+    view[h].sinks = (e.first + kN - 1) / kN;
+    view[h].last = e.hi > f.lo ? (e.hi - 1) / kN : view[h].sinks - 1;
+    if (h >= halves) view[h].last = -1;
+  }
 
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols) : "memory");
@@ -331,7 +425,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const unsigned tmem = sm.tmem_base;
+  const unsigned tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
 
   bool ok = true;
   int issued = 0;  // TMA lane: stage fills issued so far
@@ -356,7 +450,8 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         const CUtensorMap* map = (issued & 1) ? &map_v : &map_k;
         for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.kv[st]) + c * kSub, map, c * 64, kv_head, key, bar);
       }
-    } else if (warp == kMmaWarp && lane == 0 && n_blocks > 0) {
+    } else if (warp == kMmaWarp && n_blocks > 0) {
+      const unsigned leader = elect_lane();
       constexpr unsigned id_qk = kInstr<kM, kN, false>, id_pv = kInstr<kM, DP, true>;
       auto scores = [&](int h, int fill) {  // S of half h from the K tile of this fill
         const unsigned qa = smem_u32(sm.q[h]), ka = smem_u32(sm.kv[fill % kSt]);
@@ -365,38 +460,46 @@ __global__ void __launch_bounds__(kThreadsW, 1)
 #pragma unroll
           for (int k = 0; k < 4; k++)
             mma_ss(tmem + kTmemS + unsigned(h) * 128, desc_sw128(qa + c * kSub, 16) + uint64_t(2 * k), desc_sw128(ka + c * kSub, 16) + uint64_t(2 * k), id_qk,
-                   (c | k) != 0 ? 1u : 0u);
-        commit_to(smem_u32(&sm.s_full[h]));
+                   (c | k) != 0 ? 1u : 0u, leader);
+        commit_to(smem_u32(&sm.s_full[h]), leader);
       };
       auto wait_fill = [&](int fill) {
-        const bool r = mbar_wait_spin(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u);
+        const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u));
         fence_after();
         return r;
       };
-      ok = wait_fill(0);
-      for (int h = 0; h < halves && ok; h++) {
-        ok = mbar_wait_spin(smem_u32(&sm.q_full[h]), 0);
-        if (ok) scores(h, 0);
-      }
-      if (ok) commit_to(smem_u32(&sm.empty[0]));
-      for (int j = 0; j < n_blocks && ok; j++) {
+      // Block j: the products with its V, and behind each half's the scores of block j + 1, so that the tensor pipe works on
+      // one half while the other half's softmax runs.  A half passes over blocks that none of its rows sees.
+      int done[2] = {0, 0};  // blocks a half has had
+      for (int j = -1; j < n_blocks && ok; j++) {
         const int fv = 2 * j + 1, fk = 2 * j + 2;
-        if (!(ok = wait_fill(fv))) break;
-        for (int h = 0; h < halves; h++) {
-          if (!(ok = mbar_wait_spin(smem_u32(&sm.p_full[h]), unsigned(j) & 1u))) break;
-          fence_after();
-          const unsigned va = smem_u32(sm.kv[fv % kSt]);
+        if (j >= 0 && !(ok = wait_fill(fv))) break;
+        if (j + 1 < n_blocks && !(ok = wait_fill(fk))) break;
+        const int block = block_at(j), next = block_at(j + 1);
 #pragma unroll
-          for (int k = 0; k < kN / 16; k++)  // 16 keys: 8 columns of P, 2048 bytes of V
-            mma_ts(tmem + kTmemO + unsigned(h) * 128, tmem + kTmemS + unsigned(h) * 128 + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128), id_pv,
-                   (j | k) != 0 ? 1u : 0u);
-          if (h == halves - 1) commit_to(smem_u32(&sm.empty[fv % kSt]));
-          if (j + 1 < n_blocks) {
-            if (h == 0 && !(ok = wait_fill(fk))) break;
-            scores(h, fk);
-            if (h == halves - 1) commit_to(smem_u32(&sm.empty[fk % kSt]));
-          } else {
-            commit_to(smem_u32(&sm.o_full[h]));
+        for (int h = 0; h < 2; h++) {
+          if (h < halves && ok) {
+            if (j < 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.q_full[h]), 0));
+            if (j >= 0 && view[h].has(block)) {
+              const unsigned va = smem_u32(sm.kv[fv % kSt]), td = tmem + kTmemO + unsigned(h) * 128, tp = tmem + kTmemS + unsigned(h) * 128;
+              ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.p_part[h]), unsigned(done[h]) & 1u));
+              fence_after();
+#pragma unroll
+              for (int k = 0; k < kN / 16; k++) {  // 16 keys: 8 columns of P, 2048 bytes of V
+                if (k == kPart / 16 && ok) {
+                  ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.p_full[h]), unsigned(done[h]) & 1u));
+                  fence_after();
+                }
+                if (ok) mma_ts(td, tp + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128), id_pv, k > 0 || done[h] > 0 ? 1u : 0u, leader);
+              }
+              done[h]++;
+              if (ok && block == view[h].last) commit_to(smem_u32(&sm.o_full[h]), leader);
+            }
+            if (ok && h == halves - 1 && j >= 0) commit_to(smem_u32(&sm.empty[fv % kSt]), leader);
+            if (ok && j + 1 < n_blocks) {
+              if (view[h].has(next)) scores(h, fk);
+              if (h == halves - 1) commit_to(smem_u32(&sm.empty[fk % kSt]), leader);
+            }
           }
         }
       }
@@ -412,95 +515,119 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       const Seen mine = seen_by(a, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
       // the first row of the half has the nearest end, the last row the farthest window start
       const Seen h_first = seen_by(a, rh0 + shift, t.nk), h_last = seen_by(a, rh0 + rows_h - 1 + shift, t.nk);
+      const HalfView mine_blocks = h == 0 ? view[0] : view[1];
       float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), sum
+      int done = 0;                  // blocks that some row of the half sees, so far
       for (int j = 0; j < n_blocks; j++) {
+        if (!mine_blocks.has(block_at(j))) continue;
         const int key0 = block_at(j) * kN;
         const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
-        if (!(ok = mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(j) & 1u))) break;
+        if (edge) {
+          // V of this block, before the scores are there: zero what lies behind the sequence, look for values that are not
+          // finite in the rest (an exponent of all ones carries into the sign bit when one is added to it)
+          const int fv = 2 * j + 1;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u)))) break;
+          uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
+          const int there = t.nk - key0;
+          unsigned odd = 0;
+#pragma unroll
+          for (int i = 0; i < Cfg::kTileBytes / 16 / kM; i++) {
+            const uint4 x = vt[i * kM + row_h];
+            constexpr unsigned e = 0x7f807f80u, one = 0x00800080u;
+            // row of the tile: 8 chunks of 16 bytes a row, 128 rows of each 64 channels
+            const unsigned y = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
+            if ((i * (kM / 8) + (row_h >> 3)) % kN < there) odd |= y;
+          }
+          if (odd & 0x80008000u) sm.poison[h] = 1;
+          if (there < kN) {
+            for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM)
+              if ((i >> 3) % kN >= there) vt[i] = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+        }
+        // the lanes agree on the outcome, so that none is left alone at the next warp-wide instruction
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(done) & 1u)))) break;
         fence_after();
         unsigned s[4][32];
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, s[c]);
         tmem_wait_ld(s[0]);
         tmem_touch(s[1]), tmem_touch(s[2]), tmem_touch(s[3]);
         if (edge) {
+          // bit i of `below(n)`: i < n
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
           const int first = mine.first - key0, lo = mine.lo - key0, hi = mine.hi - key0;
-  #pragma unroll
-          for (int c = 0; c < 4; c++)
-  #pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const int k = 32 * c + i;
-              if (!(k < first || (k >= lo && k < hi))) s[c][i] = 0xff800000u;
-            }
-          // V of this block: zero what lies behind the sequence, look for values that are not finite in the rest
-          const int fv = 2 * j + 1;
-          if (!(ok = mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u))) break;
-          uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
-          const int there = t.nk - key0;
-          bool bad = false;
-  #pragma unroll 4
-          for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM) {
-            if (((i >> 3) & 127) < there) {
-              const uint4 x = vt[i];
-              constexpr unsigned e = 0x7f807f80u;
-              bad |= (__vcmpeq2(x.x & e, e) | __vcmpeq2(x.y & e, e) | __vcmpeq2(x.z & e, e) | __vcmpeq2(x.w & e, e)) != 0;
-            } else {
-              vt[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const unsigned see = below(first - 32 * c) | (below(hi - 32 * c) & ~below(lo - 32 * c));
+#pragma unroll
+            for (int i = 0; i < 32; i++) s[c][i] = (see >> i) & 1u ? s[c][i] : 0xff800000u;
           }
-          if (bad) sm.poison[h] = 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        float mx = -INFINITY;
-  #pragma unroll
-        for (int c = 0; c < 4; c++)
-  #pragma unroll
-          for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[c][i]));
-        const bool grow = (mx - m) * L.scale2 > kSlack;  // also the first finite score (m = -inf); false for NaN
+        float mx;
+        {
+          float part[4];
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            part[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+            for (int i = 1; i < 32; i++) part[c] = max_nan(part[c], __uint_as_float(s[c][i]));
+          }
+          mx = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
+        }
+        if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinity among the scores: the whole row is NaN
+        const bool grow = (mx - m) * L.scale2 > kSlack;          // also the first finite score (m = -inf); false for NaN
         if (__any_sync(0xffffffffu, grow)) {
           float f = 1.f;
           if (grow) {
             f = ex2_approx((m - mx) * L.scale2);
             m = mx, l *= f;
           }
-          if (j > 0) {  // every product issued so far has retired: s_full of this block was signalled behind them
-  #pragma unroll
-            for (int c = 0; c < DP / 32; c++) {
-              unsigned o[32];
-              tmem_ld32(to + 32 * c, o);
-              tmem_wait_ld(o);
-  #pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st32(to + 32 * c, o);
+          if (done > 0) {  // every product issued so far has retired: s_full of this block was signalled behind them
+#pragma unroll 1
+            for (int c = 0; c < DP / 16; c++) {
+              unsigned o[16];
+              tmem_ld16(to + 16 * c, o);
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(to + 16 * c, o);
             }
           }
         }
         const float base = m == -INFINITY ? 0.f : m * L.scale2;
-  #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          unsigned p[16];
-  #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i]), L.scale2, -base));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), L.scale2, -base));
-            l += p0 + p1;
-            p[i] = pack_bf16(p0, p1);
+        const uint64_t scale2 = pair(L.scale2, L.scale2), neg_base = pair(-base, -base);
+        uint64_t l2[2] = {0, 0};
+        if (edge) {  // a masked score has to come out as exactly 0
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            unsigned p[16];
+            exp_chunk<false>(s[c], scale2, neg_base, l2, p);
+            tmem_st16(ts + 16 * c, p);
+            if (c == kPart / 32 - 1) hand_over(&sm.p_part[h], lane);
           }
-          tmem_st16(ts + 16 * c, p);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            unsigned p[16];
+            exp_chunk<true>(s[c], scale2, neg_base, l2, p);
+            tmem_st16(ts + 16 * c, p);
+            if (c == kPart / 32 - 1) hand_over(&sm.p_part[h], lane);
+          }
         }
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(smem_u32(&sm.p_full[h]));
+        float l0, l1;
+        split(add2(l2[0], l2[1]), l0, l1);
+        l += l0 + l1;
+        hand_over(&sm.p_full[h], lane);
+        done++;
       }
       // ---- output ----
-      if (ok && n_blocks > 0) ok = mbar_wait_spin(smem_u32(&sm.o_full[h]), 0);
+      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.o_full[h]), 0);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         fence_after();
         const int64_t row = int64_t(t.q0) + rh0 + row_h;
         const bool on = row_h < rows_h;
-        if (n_blocks > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
+        if (done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
           float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 3) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
           for (int r = (warp & 3) * 32; r < min((warp & 3) * 32 + 32, rows_h); r++)
             row_attention(L, int64_t(t.q0) + rh0 + r, head, t.k0, rh0 + r + shift, t.nk, qs);
@@ -508,18 +635,18 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           const bool some = l > 0.f || l != l;
           const float f = some ? 1.f / l : 0.f;
           mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D;
-  #pragma unroll 1
+#pragma unroll 1
           for (int c = 0; c < DP / 32; c++) {
             unsigned o[32];
-            if (n_blocks > 0) {
+            if (done > 0) {
               tmem_ld32(to + 32 * c, o);
               tmem_wait_ld(o);
             }
             if (!on) continue;
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; i++) {
               float v[8];
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < 8; e++) v[e] = some ? __uint_as_float(o[8 * i + e]) * f : 0.f;
               if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
             }
