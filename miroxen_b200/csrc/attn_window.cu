@@ -7,17 +7,22 @@
 // j >= p - left (left >= 0) or j < sinks.
 //
 // Two matrix products of 4 D flops per pair with one exponential between: the tensor cores bound it, the exponentials
-// (16 per clock and SM) nearly as much.  One CTA of 384 threads holds 256 rows of one head as two halves of 128:
-//   warps 0-3, 4-7: the softmax of one half each, a thread per row.  A score tile (128 rows x 128 keys, fp32) comes from
-//                   tensor memory into registers, its row maximum, exponentials and their sum are taken there, and the
-//                   probabilities go back as bf16 (the type of V, which the product needs) over the scores they came from;
-//   warp 8:         issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory.  While one half's
-//                   softmax runs, the other half's products do;
-//   warp 9:         TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
-//   warps 10, 11:   only complete the group of four whose registers the softmax warps take over (setmaxnreg).
-// Tensor memory: S (with P in it) and O of both halves, 4 x 128 columns.  The running maximum that the exponentials use
-// moves only when it would grow by more than 2^8 (results are the same: every sum is relative to it), so O is rescaled
-// rarely, by the half's own warps, which at that point know that no product is under way on it.
+// (16 per clock and SM) nearly as much.  One CTA of 640 threads holds 256 rows of one head as two halves of 128:
+//   warps 0-7, 8-15: the softmax of one half each, two threads per row (one per 64 keys of a block).  A score tile (128 rows x
+//                   128 keys, fp32) comes from tensor memory into registers, its row maximum, exponentials and their sum
+//                   are taken there, and the probabilities go back as bf16 (the type of V, which the product needs) over
+//                   the scores they came from;
+//   warp 16, 18:    issue tcgen05.mma: S = Q K^T from shared memory (16), O += P V with P from tensor memory (18);
+//   warp 17:        TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
+//   warp 19:        only completes the group of four whose registers the softmax warps take over (setmaxnreg).
+// Tensor memory: one score tile (128 columns), which the halves use in turn, the probabilities P of each half (64) and the
+// output O of each half (128), 512 in all.  A score tile is free as soon as its half has it in registers, so the tensor pipe
+// makes the next one, and the products with V, while the softmax runs: S0 | S1 | S0' P0 V | S1' P1 V | ...  Nothing goes
+// round in a chain but the softmax of a half, which has a whole turn of the tensor pipe for itself.  (With the
+// probabilities written over their scores, two score tiles fit, but then a half's next scores have to wait for its product
+// with V: measured 3900 clocks per turn of 4 products of 128^3 against XX here.)
+// The running maximum that the exponentials use moves only when it would grow by more than 2^8 (results are the same:
+// every sum is relative to it), so O is rescaled rarely, by the half's own warps, once its products so far have retired.
 // Blocks of 128 keys outside of every row's view are not visited; only blocks at the edge of some row's view pay for the
 // mask.  There, what lies out of view must not reach 0 * v: value rows behind the sequence are zeroed in shared memory, and
 // if any other value of the block is not finite the rows are taken again by a plain loop (row_attention) that never touches
@@ -37,41 +42,31 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnLaunch {
   MxkAttnArgs a;
-  int group;     // query heads per key head
-  float scale2;  // scale * log2(e)
+  int left, right, sinks;  // a's, no bound as kFar
+  int group;               // query heads per key head
+  float scale2;            // scale * log2(e)
   int* err;
 };
-
-// First row of sequence b, held inside [0, rows] and not before `least` whatever the array holds.
-__device__ __forceinline__ int cu_at(const int32_t* cu, int b, int64_t rows, int least, int* err) {
-  const int v = cu[b];
-  if (v < least || v > rows) {
-    if (err) atomicExch(err, kErrBadIndex);
-    return v < least ? least : int(rows);
-  }
-  return v;
-}
+constexpr int kFar = 1 << 30;  // rows and keys are fewer, so that positions and bounds add up in 32 bits
 
 // Keys that a row at position p of a sequence of nk keys sees: [0, first) and [lo, hi).
 struct Seen {
   int first, lo, hi;
 };
-__device__ __forceinline__ Seen seen_by(const MxkAttnArgs& a, int64_t p, int nk) {
-  Seen s{0, 0, nk};
-  if (a.right >= 0 && p + a.right + 1 < nk) s.hi = p + a.right + 1 < 0 ? 0 : int(p + a.right + 1);
-  if (a.left >= 0 && p - a.left > 0) s.lo = p - a.left > nk ? nk : int(p - a.left);
-  s.first = a.sinks < s.lo ? int(a.sinks) : s.lo;
-  if (s.first > s.hi) s.first = s.hi;
-  if (s.lo > s.hi) s.lo = s.hi;
+__device__ __forceinline__ Seen seen_by(const AttnLaunch& L, int p, int nk) {
+  Seen s;
+  s.hi = max(0, min(nk, p + L.right + 1));
+  s.lo = max(0, min(s.hi, p - L.left));
+  s.first = min(L.sinks, s.lo);
   return s;
 }
 
 // One row and head by one warp, 32 keys at a time: a lane takes a key's product with q, then the warp adds the keys'
 // values, each lane holding channels 2 lane, 2 lane + 1, + 64.  `qs`: the warp's 128 floats of shared memory.
-__device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k0, int64_t p, int nk, float* qs) {
+__device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k0, int p, int nk, float* qs) {
   const MxkAttnArgs& a = L.a;
   const int lane = threadIdx.x & 31, D = a.D, g = h / L.group;
-  const Seen seen = seen_by(a, p, nk);
+  const Seen seen = seen_by(L, p, nk);
   const mxk_bf16* q = a.q + row * a.q_stride + int64_t(h) * D;
   __syncwarp();
   for (int d = lane; d < D; d += 32) qs[d] = __uint_as_float(unsigned(q[d]) << 16);
@@ -133,13 +128,13 @@ __device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------
 
 constexpr int kM = 128, kN = 128;              // rows of a half, keys of a block
-constexpr int kMmaWarp = 8, kTmaWarp = 9, kThreadsW = 384;
+constexpr int kScoreWarp = 16, kTmaWarp = 17, kValueWarp = 18, kThreadsW = 640;
 constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channel tile
-// Registers a thread: 384 x 168 at launch; a softmax thread holds a row of 128 scores, the warps of the third group need few.
-constexpr int kRegsSoft = 208, kRegsOther = 88;
-static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
-constexpr unsigned kTmemS = 0, kTmemO = 256, kTmemCols = 512;
-constexpr int kPart = 96;                      // keys after which the first part of the probabilities is handed over
+// Registers a thread: 640 x 96 at launch; a softmax thread holds 64 scores, the others need fewer.
+constexpr int kRegsSoft = 104, kRegsOther = 64;
+static_assert(512 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 96, "the groups' registers are those of the launch");
+constexpr unsigned kTmemS = 0, kTmemP = 128, kTmemO = 256, kTmemCols = 512;  // S, 2 x 64 of P, 2 x 128 of O
+constexpr int kPart = 64;                      // keys of a block that one of a row's two threads takes
 constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
 
 template <int DP>
@@ -153,10 +148,11 @@ template <int DP>
 struct __align__(1024) WindowSmem {
   unsigned char q[2][WindowCfg<DP>::kTileBytes];
   unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
-  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], p_part[2], p_full[2], o_full[2];
+  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2], max_read[2];
   unsigned tmem_base;
   int poison[2];  // a value that is not finite lies in a block at the edge of the half's view
-  int scan[kThreadsW / 32], found[4];
+  int scan[kThreadsW / 32], found[6];
+  float row_max[2][2][kM];  // [half][thread of the row][row]: what the two threads of a row tell each other
 };
 
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned bar) {
@@ -251,66 +247,55 @@ __device__ __forceinline__ void hand_over(unsigned long long* bar, int lane) {
   if (lane == 0) mbar_arrive1(smem_u32(bar));
 }
 
-// Pairs of fp32 operations (one issue slot for two).
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {  // NaN if one of them is
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of a pair on the multiply-add pipe, for -126 <= x < 127: x = n + f, |f| <= 1/2, n by adding and taking away 1.5 * 2^23
+// 2^x of N values on the multiply-add pipe, for -126 <= x < 127: x = n + f, |f| <= 1/2, n by adding and taking away 1.5 * 2^23
 // (the integer then stands in the low bits), 2^f by a polynomial of degree 5 fitted to the least relative error on
 // [-1/2, 1/2] (7.5e-8, below the hardware's 2^x), n added to its exponent.
-__device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
-  const uint64_t magic = pair(12582912.f, 12582912.f), unmagic = pair(-12582912.f, -12582912.f), minus = pair(-1.f, -1.f);
-  const uint64_t r = add2(x, magic), n = add2(r, unmagic), f = fma2(n, minus, x);
-  uint64_t p = fma2(f, pair(1.3276472454890609e-3f, 1.3276472454890609e-3f), pair(9.675540961325169e-3f, 9.675540961325169e-3f));
-  p = fma2(p, f, pair(5.550713092088699e-2f, 5.550713092088699e-2f));
-  p = fma2(p, f, pair(0.24022120237350464f, 0.24022120237350464f));
-  p = fma2(p, f, pair(0.6931469440460205f, 0.6931469440460205f));
-  p = fma2(p, f, pair(1.0000001192092896f, 1.0000001192092896f));
-  float pl, ph, rl, rh;
-  split(p, pl, ph), split(r, rl, rh);
-  lo = __uint_as_float(__float_as_uint(pl) + (__float_as_uint(rl) << 23));
-  hi = __uint_as_float(__float_as_uint(ph) + (__float_as_uint(rh) << 23));
+template <int N>
+__device__ __forceinline__ void exp2_poly(float (&x)[N]) {
+  constexpr float c[6] = {1.3276472454890609e-3f, 9.675540961325169e-3f, 5.550713092088699e-2f, 0.24022120237350464f, 0.6931469440460205f, 1.0000001192092896f};
+  float r[N], f[N], p[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = fmaxf(x[i], -126.f), r[i] = x[i] + 12582912.f;
+#pragma unroll
+  for (int i = 0; i < N; i++) f[i] = x[i] - (r[i] - 12582912.f), p[i] = fmaf(f[i], c[0], c[1]);
+#pragma unroll
+  for (int k = 2; k < 6; k++)
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fmaf(p[i], f[i], c[k]);
+#pragma unroll
+  for (int i = 0; i < N; i++) x[i] = __uint_as_float(__float_as_uint(p[i]) + (__float_as_uint(r[i]) << 23));
 }
-// Of every eight pairs of scores this many take their 2^x on the multiply-add pipe, the others on the special-function unit.
 #ifndef MXK_POLY
 #define MXK_POLY 0
 #endif
-constexpr int kPolyPairs = MXK_POLY;
+constexpr int kPoly = MXK_POLY;  // of 32 scores this many take their 2^x on the multiply-add pipe
 
-// Probabilities of 32 scores: p = 2^(s * scale2 - base), their sum into l2 (two partial sums), rounded to bf16 in pairs.
+// Probabilities of 32 scores: p = 2^(s * scale2 - base), their sum into l (four partial sums), rounded to bf16 in pairs.
 template <bool POLY>
-__device__ __forceinline__ void exp_chunk(const unsigned (&s)[32], uint64_t scale2, uint64_t neg_base, uint64_t (&l2)[2], unsigned (&p)[16]) {
+__device__ __forceinline__ void exp_chunk(const unsigned (&s)[32], float scale2, float base, float (&l)[4], unsigned (&p)[16]) {
+  constexpr int N = POLY ? kPoly : 0;
+  float x[32];
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, neg_base);
-    float lo, hi, p0, p1;
-    split(x, lo, hi);
-    if (POLY && (i % 8) * kPolyPairs % 8 + kPolyPairs >= 8) {
-      exp2_pair(pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f)), p0, p1);
-    } else {
-      p0 = ex2_approx(lo), p1 = ex2_approx(hi);
-    }
-    l2[i & 1] = add2(l2[i & 1], pair(p0, p1));
-    p[i] = pack_bf16(p0, p1);
+  for (int i = 0; i < 32; i++) x[i] = fmaf(__uint_as_float(s[i]), scale2, -base);
+  if constexpr (N > 0) {
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = x[i];
+    exp2_poly(y);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = y[i];
   }
+#pragma unroll
+  for (int i = N; i < 32; i++) x[i] = ex2_approx(x[i]);
+#pragma unroll
+  for (int i = 0; i < 32; i++) l[i & 3] += x[i];
+#pragma unroll
+  for (int i = 0; i < 16; i++) p[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
 }
 
 struct WindowLaunch {
@@ -334,14 +319,18 @@ __device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int want,
     t.rows = min(tile_rows, t.nq - t.r0);
     return t;
   }
-  // thread t counts a contiguous share of the sequences
+  // thread t counts a contiguous share of the sequences; the ends of its first one (its only one, mostly) stay in registers
   const int n = a.n_seqs, share = (n + kThreadsW - 1) / kThreadsW, b0 = min(n, tid * share), b1 = min(n, b0 + share);
-  auto tiles = [&](int b) {
-    const int q0 = cu_at(a.cu_q, b, a.q_rows, 0, W.L.err);
-    return (cu_at(a.cu_q, b + 1, a.q_rows, q0, W.L.err) - q0 + tile_rows - 1) / tile_rows;
+  int mine = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  auto ends = [&](int b) {
+    const int x0 = a.cu_q[b], x1 = a.cu_q[b + 1], y0 = a.cu_k[b], y1 = a.cu_k[b + 1];
+    // held inside the arrays and in order whatever they hold
+    q0 = max(0, min(x0, int(a.q_rows))), q1 = max(q0, min(x1, int(a.q_rows)));
+    k0 = max(0, min(y0, int(a.k_rows))), k1 = max(k0, min(y1, int(a.k_rows)));
+    if ((q0 != x0 || q1 != x1 || k0 != y0 || k1 != y1) && W.L.err) atomicExch(W.L.err, kErrBadIndex);
+    return (q1 - q0 + tile_rows - 1) / tile_rows;
   };
-  int mine = 0;
-  for (int b = b0; b < b1; b++) mine += tiles(b);
+  for (int b = b1 - 1; b >= b0; b--) mine += ends(b);
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -349,21 +338,19 @@ __device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int want,
     if (lane >= o) incl += x;
   }
   if (lane == 31) scan[warp] = incl;
-  if (tid == 0) found[0] = -1;
+  if (tid == 0) found[5] = 0;
   __syncthreads();
   int at = incl - mine;
   for (int w = 0; w < warp; w++) at += scan[w];
   if (want >= at && want < at + mine) {
     int b = b0;
-    for (int k = tiles(b); want >= at + k; k = tiles(b)) at += k, b++;
-    found[0] = b, found[1] = want - at;
+    if (share > 1)
+      for (int k = ends(b); want >= at + k; k = ends(b)) at += k, b++;
+    found[0] = q0, found[1] = q1 - q0, found[2] = k0, found[3] = k1 - k0, found[4] = (want - at) * tile_rows, found[5] = 1;
   }
   __syncthreads();
-  const int b = found[0];
-  if (b < 0) return t;
-  t.q0 = cu_at(a.cu_q, b, a.q_rows, 0, W.L.err), t.nq = cu_at(a.cu_q, b + 1, a.q_rows, t.q0, W.L.err) - t.q0;
-  t.k0 = cu_at(a.cu_k, b, a.k_rows, 0, W.L.err), t.nk = cu_at(a.cu_k, b + 1, a.k_rows, t.k0, W.L.err) - t.k0;
-  t.r0 = found[1] * tile_rows;
+  if (!found[5]) return t;
+  t.q0 = found[0], t.nq = found[1], t.k0 = found[2], t.nk = found[3], t.r0 = found[4];
   t.rows = min(tile_rows, t.nq - t.r0);
   return t;
 }
@@ -374,20 +361,23 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                   const __grid_constant__ WindowLaunch W) {
   using Cfg = WindowCfg<DP>;
   constexpr int kSt = Cfg::kStages;
-  extern __shared__ unsigned char smem_raw[];
-  WindowSmem<DP>& sm = *reinterpret_cast<WindowSmem<DP>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // There is no room to align the tiles by hand; without static shared memory the dynamic part starts on a 1 KB boundary.
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  WindowSmem<DP>& sm = *reinterpret_cast<WindowSmem<DP>*>(smem_raw);
   const AttnLaunch& L = W.L;
   const MxkAttnArgs& a = L.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  // the tiles at the end of a causal sequence have the most keys: they start first
-  const int head = int(blockIdx.x) % a.H, want = W.max_tiles - 1 - int(blockIdx.x) / a.H, kv_head = head / L.group;
+  // Head by head, so that the CTAs at work read the keys of few heads and at about the same time; the tiles at the end of a
+  // causal sequence, which have the most keys, first.
+  const int head = int(blockIdx.x) / W.max_tiles, want = W.max_tiles - 1 - int(blockIdx.x) % W.max_tiles, kv_head = head / L.group;
 
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.o_full[i]), 1);
-      mbar_init(smem_u32(&sm.p_part[i]), 4), mbar_init(smem_u32(&sm.p_full[i]), 4);
+      mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.pv_done[i]), 1);
+      mbar_init(smem_u32(&sm.p_full[i]), 8), mbar_init(smem_u32(&sm.max_read[i]), 8);
       sm.poison[i] = 0;
     }
+    mbar_init(smem_u32(&sm.s_free), 8);
     for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -395,11 +385,15 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   pdl_wait();
   const WindowTile t = find_tile(W, want, sm.scan, sm.found);
   if (t.rows <= 0) return;  // the whole CTA
+  if (smem_u32(smem_raw) & 1023u) {  // never seen; nothing is computed on tiles that the swizzle would not fit
+    if (tid == 0 && L.err) atomicExch(L.err, kErrBulkTimeout);
+    return;
+  }
   const int halves = t.rows > kM ? 2 : 1;
 
   // blocks of keys that some row of the tile sees: n_sink from the front, the others from block wb0 on
-  const int64_t shift = int64_t(t.nk) - t.nq;  // a row's position is its number + shift
-  const Seen s_first = seen_by(a, t.r0 + shift, t.nk), s_last = seen_by(a, t.r0 + t.rows - 1 + shift, t.nk);
+  const int shift = t.nk - t.nq;  // a row's position is its number + shift
+  const Seen s_first = seen_by(L, t.r0 + shift, t.nk), s_last = seen_by(L, t.r0 + t.rows - 1 + shift, t.nk);
   const int wb0 = s_first.lo / kN, wb1 = s_last.hi > s_first.lo ? (s_last.hi + kN - 1) / kN : wb0;
   const int n_sink = min((s_last.first + kN - 1) / kN, wb0);
   const int n_blocks = n_sink + wb1 - wb0;
@@ -409,16 +403,18 @@ __global__ void __launch_bounds__(kThreadsW, 1)
     int sinks, from, last;
     __device__ __forceinline__ bool has(int block) const { return block <= last && (block < sinks || block >= from); }
   } view[2];
+  int first_block[2];  // its place in the order of the tile's blocks
 #pragma unroll
   for (int h = 0; h < 2; h++) {
-    const Seen f = seen_by(a, t.r0 + h * kM + shift, t.nk), e = seen_by(a, t.r0 + min((h + 1) * kM, t.rows) - 1 + shift, t.nk);
+    const Seen f = seen_by(L, t.r0 + h * kM + shift, t.nk), e = seen_by(L, t.r0 + min((h + 1) * kM, t.rows) - 1 + shift, t.nk);
     view[h].from = f.lo / kN;
     view[h].sinks = (e.first + kN - 1) / kN;
     view[h].last = e.hi > f.lo ? (e.hi - 1) / kN : view[h].sinks - 1;
+    first_block[h] = view[h].sinks > 0 ? 0 : view[h].from - wb0 + n_sink;
     if (h >= halves) view[h].last = -1;
   }
 
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -429,7 +425,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
 
   bool ok = true;
   int issued = 0;  // TMA lane: stage fills issued so far
-  if (warp >= kMmaWarp) {
+  if (warp >= kScoreWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kTmaWarp && lane == 0 && n_blocks > 0) {
       for (int h = 0; h < halves; h++) {
@@ -450,131 +446,149 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         const CUtensorMap* map = (issued & 1) ? &map_v : &map_k;
         for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.kv[st]) + c * kSub, map, c * 64, kv_head, key, bar);
       }
-    } else if (warp == kMmaWarp && n_blocks > 0) {
+    } else if ((warp == kScoreWarp || warp == kValueWarp) && n_blocks > 0) {
       const unsigned leader = elect_lane();
-      constexpr unsigned id_qk = kInstr<kM, kN, false>, id_pv = kInstr<kM, DP, true>;
-      auto scores = [&](int h, int fill) {  // S of half h from the K tile of this fill
-        const unsigned qa = smem_u32(sm.q[h]), ka = smem_u32(sm.kv[fill % kSt]);
-#pragma unroll
-        for (int c = 0; c < Cfg::kSubs; c++)
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            mma_ss(tmem + kTmemS + unsigned(h) * 128, desc_sw128(qa + c * kSub, 16) + uint64_t(2 * k), desc_sw128(ka + c * kSub, 16) + uint64_t(2 * k), id_qk,
-                   (c | k) != 0 ? 1u : 0u, leader);
-        commit_to(smem_u32(&sm.s_full[h]), leader);
-      };
-      auto wait_fill = [&](int fill) {
-        const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fill % kSt]), unsigned(fill / kSt) & 1u));
+      auto wait = [&](unsigned long long* bar, int phase) {
+        const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(bar), unsigned(phase) & 1u));
         fence_after();
         return r;
       };
-      // Block j: the products with its V, and behind each half's the scores of block j + 1, so that the tensor pipe works on
-      // one half while the other half's softmax runs.  A half passes over blocks that none of its rows sees.
-      int done[2] = {0, 0};  // blocks a half has had
-      for (int j = -1; j < n_blocks && ok; j++) {
-        const int fv = 2 * j + 1, fk = 2 * j + 2;
-        if (j >= 0 && !(ok = wait_fill(fv))) break;
-        if (j + 1 < n_blocks && !(ok = wait_fill(fk))) break;
-        const int block = block_at(j), next = block_at(j + 1);
+      // A half passes over blocks that none of its rows sees.
+      if (warp == kScoreWarp) {
+        int made = 0;  // score tiles so far
+        for (int j = 0; j < n_blocks && ok; j++) {
+          const int block = block_at(j), fill = 2 * j;
+          ok = wait(&sm.full[fill % kSt], fill / kSt);
+          const unsigned ka = smem_u32(sm.kv[fill % kSt]);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          if (h < halves && ok) {
-            if (j < 0) ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.q_full[h]), 0));
-            if (j >= 0 && view[h].has(block)) {
-              const unsigned va = smem_u32(sm.kv[fv % kSt]), td = tmem + kTmemO + unsigned(h) * 128, tp = tmem + kTmemS + unsigned(h) * 128;
-              ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.p_part[h]), unsigned(done[h]) & 1u));
-              fence_after();
+          for (int h = 0; h < 2; h++) {
+            if (h >= halves || !ok || !view[h].has(block)) continue;
+            if (j == first_block[h]) ok = wait(&sm.q_full[h], 0);
+            if (ok && made > 0) ok = wait(&sm.s_free, made - 1);  // the tile before this one is in its half's registers
+            if (!ok) continue;
+            const unsigned qa = smem_u32(sm.q[h]);
 #pragma unroll
-              for (int k = 0; k < kN / 16; k++) {  // 16 keys: 8 columns of P, 2048 bytes of V
-                if (k == kPart / 16 && ok) {
-                  ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.p_full[h]), unsigned(done[h]) & 1u));
-                  fence_after();
-                }
-                if (ok) mma_ts(td, tp + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128), id_pv, k > 0 || done[h] > 0 ? 1u : 0u, leader);
-              }
-              done[h]++;
-              if (ok && block == view[h].last) commit_to(smem_u32(&sm.o_full[h]), leader);
-            }
-            if (ok && h == halves - 1 && j >= 0) commit_to(smem_u32(&sm.empty[fv % kSt]), leader);
-            if (ok && j + 1 < n_blocks) {
-              if (view[h].has(next)) scores(h, fk);
-              if (h == halves - 1) commit_to(smem_u32(&sm.empty[fk % kSt]), leader);
-            }
+            for (int c = 0; c < Cfg::kSubs; c++)
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                mma_ss(tmem + kTmemS, desc_sw128(qa + c * kSub, 16) + uint64_t(2 * k), desc_sw128(ka + c * kSub, 16) + uint64_t(2 * k),
+                       kInstr<kM, kN, false>, (c | k) != 0 ? 1u : 0u, leader);
+            commit_to(smem_u32(&sm.s_full[h]), leader);
+            made++;
           }
+          if (ok) commit_to(smem_u32(&sm.empty[fill % kSt]), leader);
+        }
+      } else {
+        int done[2] = {0, 0};  // blocks a half has had
+        for (int j = 0; j < n_blocks && ok; j++) {
+          const int block = block_at(j), fill = 2 * j + 1;
+          ok = wait(&sm.full[fill % kSt], fill / kSt);
+          const unsigned va = smem_u32(sm.kv[fill % kSt]);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (h >= halves || !ok || !view[h].has(block)) continue;
+            ok = wait(&sm.p_full[h], done[h]);
+            if (!ok) continue;
+#pragma unroll
+            for (int k = 0; k < kN / 16; k++)  // 16 keys: 8 columns of P, 2048 bytes of V
+              mma_ts(tmem + kTmemO + unsigned(h) * 128, tmem + kTmemP + unsigned(h) * 64 + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128),
+                     kInstr<kM, DP, true>, k > 0 || done[h] > 0 ? 1u : 0u, leader);
+            commit_to(smem_u32(&sm.pv_done[h]), leader);
+            done[h]++;
+          }
+          if (ok) commit_to(smem_u32(&sm.empty[fill % kSt]), leader);
         }
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
-    if ((warp >> 2) < halves) {
-      // ---- softmax of half h: thread (warp & 3) * 32 + lane owns that row ----
-      const int h = warp >> 2, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
-      const int rows_h = min(kM, t.rows - h * kM);
+    if ((warp >> 3) < halves) {
+      // ---- softmax of half h: thread (warp & 3) * 32 + lane of either group of four warps owns that row's 64 keys `sub` ----
+      const int h = warp >> 3, sub = (warp >> 2) & 1, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
+      const int rows_h = min(kM, t.rows - h * kM), in_half = (warp & 7) * 32 + lane;
       const unsigned lanes = unsigned((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + lanes + kTmemS + unsigned(h) * 128, to = tmem + lanes + kTmemO + unsigned(h) * 128;
-      const Seen mine = seen_by(a, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
+      const unsigned ts = tmem + lanes + kTmemS + unsigned(sub) * kPart, tp = tmem + lanes + kTmemP + unsigned(h) * 64 + unsigned(sub) * 32;
+      const unsigned to = tmem + lanes + kTmemO + unsigned(h) * 128 + unsigned(sub) * (DP / 2);
+      const Seen mine = seen_by(L, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
       // the first row of the half has the nearest end, the last row the farthest window start
-      const Seen h_first = seen_by(a, rh0 + shift, t.nk), h_last = seen_by(a, rh0 + rows_h - 1 + shift, t.nk);
-      const HalfView mine_blocks = h == 0 ? view[0] : view[1];
-      float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), sum
+      const Seen h_first = seen_by(L, rh0 + shift, t.nk), h_last = seen_by(L, rh0 + rows_h - 1 + shift, t.nk);
+      const HalfView blocks = h == 0 ? view[0] : view[1];
+      auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + h) : "memory"); };  // the half's eight warps
+      float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), this thread's part of the sum
       int done = 0;                  // blocks that some row of the half sees, so far
       for (int j = 0; j < n_blocks; j++) {
-        if (!mine_blocks.has(block_at(j))) continue;
-        const int key0 = block_at(j) * kN;
+        const int block = block_at(j);
+        if (!blocks.has(block)) continue;
+        const int key0 = block * kN;
         const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
+        // A wait that runs out does not leave the loop: the half's warps go on meeting, without waiting for anything else.
+        // The lanes of a warp agree on the outcome.
         if (edge) {
           // V of this block, before the scores are there: zero what lies behind the sequence, look for values that are not
           // finite in the rest (an exponent of all ones carries into the sign bit when one is added to it)
           const int fv = 2 * j + 1;
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u)))) break;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u));
           uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
           const int there = t.nk - key0;
           unsigned odd = 0;
+          if (ok) {
 #pragma unroll
-          for (int i = 0; i < Cfg::kTileBytes / 16 / kM; i++) {
-            const uint4 x = vt[i * kM + row_h];
-            constexpr unsigned e = 0x7f807f80u, one = 0x00800080u;
-            // row of the tile: 8 chunks of 16 bytes a row, 128 rows of each 64 channels
-            const unsigned y = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
-            if ((i * (kM / 8) + (row_h >> 3)) % kN < there) odd |= y;
+            for (int i = 0; i < Cfg::kTileBytes / 16 / (2 * kM); i++) {
+              const uint4 x = vt[i * 2 * kM + in_half];
+              constexpr unsigned e = 0x7f807f80u, one = 0x00800080u;
+              const unsigned y = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
+              // row of the tile: 8 chunks of 16 bytes a row, 128 rows of each 64 channels
+              if (((i * 2 * kM + in_half) >> 3) % kN < there) odd |= y;
+            }
           }
           if (odd & 0x80008000u) sm.poison[h] = 1;
-          if (there < kN) {
-            for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM)
+          if (ok && there < kN) {
+            for (int i = in_half; i < Cfg::kTileBytes / 16; i += 2 * kM)
               if ((i >> 3) % kN >= there) vt[i] = make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
-        // the lanes agree on the outcome, so that none is left alone at the next warp-wide instruction
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(done) & 1u)))) break;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(done) & 1u));
         fence_after();
-        unsigned s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, s[c]);
+        unsigned s[2][32];
+        tmem_ld32(ts, s[0]);
+        tmem_ld32(ts + 32, s[1]);
         tmem_wait_ld(s[0]);
-        tmem_touch(s[1]), tmem_touch(s[2]), tmem_touch(s[3]);
+        tmem_touch(s[1]);
+        fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive1(smem_u32(&sm.s_free));  // the other half's scores may come
         if (edge) {
-          // bit i of `below(n)`: i < n
+          // bit i of below(n): i < n
           auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-          const int first = mine.first - key0, lo = mine.lo - key0, hi = mine.hi - key0;
+          const int k0 = key0 + sub * kPart;
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const unsigned see = below(first - 32 * c) | (below(hi - 32 * c) & ~below(lo - 32 * c));
+          for (int c = 0; c < 2; c++) {
+            const unsigned see = below(mine.first - k0 - 32 * c) | (below(mine.hi - k0 - 32 * c) & ~below(mine.lo - k0 - 32 * c));
 #pragma unroll
             for (int i = 0; i < 32; i++) s[c][i] = (see >> i) & 1u ? s[c][i] : 0xff800000u;
           }
         }
         float mx;
         {
-          float part[4];
+          float part[2];
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            part[c] = __uint_as_float(s[c][0]);
+          for (int c = 0; c < 2; c++) {
+            part[c] = max_nan(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), __uint_as_float(s[c][2]));
 #pragma unroll
-            for (int i = 1; i < 32; i++) part[c] = max_nan(part[c], __uint_as_float(s[c][i]));
+            for (int i = 3; i < 31; i += 2) part[c] = max_nan(part[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
           }
-          mx = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
+          mx = max_nan(part[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+          mx = max_nan(mx, part[1], part[1]);
         }
+        // The row's maximum is both threads'.  A slot is written again only when the last block's has been read.
+        if (done > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.max_read[h]), unsigned(done - 1) & 1u));
+        sm.row_max[h][sub][row_h] = mx;
+        meet();
+        const float other = sm.row_max[h][sub ^ 1][row_h];
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(smem_u32(&sm.max_read[h]));
+        mx = max_nan(mx, other, other);
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinity among the scores: the whole row is NaN
         const bool grow = (mx - m) * L.scale2 > kSlack;          // also the first finite score (m = -inf); false for NaN
         if (__any_sync(0xffffffffu, grow)) {
@@ -583,9 +597,11 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             f = ex2_approx((m - mx) * L.scale2);
             m = mx, l *= f;
           }
-          if (done > 0) {  // every product issued so far has retired: s_full of this block was signalled behind them
+          if (done > 0 && ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u));
+            fence_after();
 #pragma unroll 1
-            for (int c = 0; c < DP / 16; c++) {
+            for (int c = 0; c < DP / 32; c++) {
               unsigned o[16];
               tmem_ld16(to + 16 * c, o);
 #pragma unroll
@@ -595,48 +611,55 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           }
         }
         const float base = m == -INFINITY ? 0.f : m * L.scale2;
-        const uint64_t scale2 = pair(L.scale2, L.scale2), neg_base = pair(-base, -base);
-        uint64_t l2[2] = {0, 0};
+        float l4[4] = {0.f, 0.f, 0.f, 0.f};
+        // P is the product's until it has retired
+        auto wait_p = [&]() {
+          if (done > 0 && ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u));
+            fence_after();
+          }
+        };
         if (edge) {  // a masked score has to come out as exactly 0
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
+          for (int c = 0; c < 2; c++) {
             unsigned p[16];
-            exp_chunk<false>(s[c], scale2, neg_base, l2, p);
-            tmem_st16(ts + 16 * c, p);
-            if (c == kPart / 32 - 1) hand_over(&sm.p_part[h], lane);
+            exp_chunk<false>(s[c], L.scale2, base, l4, p);
+            if (c == 0) wait_p();
+            tmem_st16(tp + 16 * c, p);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
+          for (int c = 0; c < 2; c++) {
             unsigned p[16];
-            exp_chunk<true>(s[c], scale2, neg_base, l2, p);
-            tmem_st16(ts + 16 * c, p);
-            if (c == kPart / 32 - 1) hand_over(&sm.p_part[h], lane);
+            exp_chunk<true>(s[c], L.scale2, base, l4, p);
+            if (c == 0) wait_p();
+            tmem_st16(tp + 16 * c, p);
           }
         }
-        float l0, l1;
-        split(add2(l2[0], l2[1]), l0, l1);
-        l += l0 + l1;
-        hand_over(&sm.p_full[h], lane);
+        if (ok) hand_over(&sm.p_full[h], lane);
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         done++;
       }
-      // ---- output ----
-      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.o_full[h]), 0);
+      // ---- output: each of a row's two threads has half of the channels ----
+      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u);
       ok = __all_sync(0xffffffffu, ok);
+      sm.row_max[h][sub][row_h] = l;
+      meet();
+      l += sm.row_max[h][sub ^ 1][row_h];
       if (ok) {
         fence_after();
         const int64_t row = int64_t(t.q0) + rh0 + row_h;
         const bool on = row_h < rows_h;
         if (done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
-          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 3) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
-          for (int r = (warp & 3) * 32; r < min((warp & 3) * 32 + 32, rows_h); r++)
+          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 7) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
+          for (int r = (warp & 7) * 16; r < min((warp & 7) * 16 + 16, rows_h); r++)
             row_attention(L, int64_t(t.q0) + rh0 + r, head, t.k0, rh0 + r + shift, t.nk, qs);
         } else {
           const bool some = l > 0.f || l != l;
           const float f = some ? 1.f / l : 0.f;
-          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D;
+          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D + sub * (DP / 2);
 #pragma unroll 1
-          for (int c = 0; c < DP / 32; c++) {
+          for (int c = 0; c < DP / 64; c++) {
             unsigned o[32];
             if (done > 0) {
               tmem_ld32(to + 32 * c, o);
@@ -648,10 +671,10 @@ __global__ void __launch_bounds__(kThreadsW, 1)
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; e++) v[e] = some ? __uint_as_float(o[8 * i + e]) * f : 0.f;
-              if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
+              if (sub * (DP / 2) + 32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
             }
           }
-          if (on && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
+          if (on && sub == 0 && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
         }
       }
     }
@@ -668,7 +691,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
     }
     __syncthreads();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
@@ -716,7 +739,7 @@ int launch_window(const char* name, WindowLaunch& W, cudaStream_t s) {
   if (int rc = make_map(name, &mk, a.k_rows > 0 ? a.k : a.q, a.k_rows > 0 ? a.k_rows : 1, a.k_rows > 0 ? a.Hkv : 1, a.D, a.k_stride)) return rc;
   if (int rc = make_map(name, &mv, a.k_rows > 0 ? a.v : a.q, a.k_rows > 0 ? a.k_rows : 1, a.k_rows > 0 ? a.Hkv : 1, a.D, a.v_stride)) return rc;
   auto k = window_kernel<DP>;
-  const size_t smem = sizeof(WindowSmem<DP>) + 1024;
+  const size_t smem = sizeof(WindowSmem<DP>);
   const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return fail(MXK_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(e));
   const int64_t ctas = int64_t(W.max_tiles) * a.H;
@@ -745,7 +768,7 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
     return fail(MXK_ERR_INVALID_ARG, "%s: head dimension %d must be a multiple of 8 and at most %d", name, a.D, MXK_ATTN_MAX_HEAD_DIM);
   if ((a.cu_q == nullptr) != (a.cu_k == nullptr) || (!a.cu_q && a.n_seqs != 1))
     return fail(MXK_ERR_INVALID_ARG, "%s: cu_q and cu_k come together, and several sequences need them (n_seqs=%d)", name, a.n_seqs);
-  if (a.q_rows >= (int64_t(1) << 31) || a.k_rows >= (int64_t(1) << 31))
+  if (a.q_rows >= kFar || a.k_rows >= kFar)
     return fail(MXK_ERR_TOO_LARGE, "%s: q_rows=%lld k_rows=%lld", name, (long long)a.q_rows, (long long)a.k_rows);
   if (a.q_stride % 8 != 0 || a.k_stride % 8 != 0 || a.v_stride % 8 != 0 || a.out_stride % 8 != 0)
     return fail(MXK_ERR_INVALID_ARG, "%s: strides must be multiples of 8", name);
@@ -759,9 +782,9 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   L.group = a.H / a.Hkv;
   L.scale2 = a.scale * kLog2e;
   L.err = device_error_word();
-  // bounds that no position reaches
-  if (L.a.left >= (int64_t(1) << 32)) L.a.left = -1;
-  if (L.a.right >= (int64_t(1) << 32)) L.a.right = -1;
+  L.left = a.left < 0 || a.left > kFar ? kFar : int(a.left);
+  L.right = a.right < 0 || a.right > kFar ? kFar : int(a.right);
+  L.sinks = a.sinks > kFar ? kFar : int(a.sinks);
   WindowLaunch W{L, 2, 0};
   // at most one tile per sequence is not full
   auto tiles = [&](int rows) { return a.n_seqs == 1 ? ceil_div(a.q_rows, rows) : a.q_rows / rows + (a.n_seqs < a.q_rows ? a.n_seqs : a.q_rows); };
