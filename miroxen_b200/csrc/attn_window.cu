@@ -7,14 +7,13 @@
 // j >= p - left (left >= 0) or j < sinks.
 //
 // Two matrix products of 4 D flops per pair with one exponential between: the tensor cores bound it, the exponentials
-// (16 per clock and SM) nearly as much.  One CTA of 640 threads holds 256 rows of one head as two halves of 128:
-//   warps 0-7, 8-15: the softmax of one half each, two threads per row (one per 64 keys of a block).  A score tile (128 rows x
-//                   128 keys, fp32) comes from tensor memory into registers, its row maximum, exponentials and their sum
-//                   are taken there, and the probabilities go back as bf16 (the type of V, which the product needs) over
-//                   the scores they came from;
-//   warp 16, 18:    issue tcgen05.mma: S = Q K^T from shared memory (16), O += P V with P from tensor memory (18);
-//   warp 17:        TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
-//   warp 19:        only completes the group of four whose registers the softmax warps take over (setmaxnreg).
+// (16 per clock and SM) nearly as much.  One CTA of 384 threads holds 256 rows of one head as two halves of 128:
+//   warps 0-3, 4-7: the softmax of one half each, a thread per row.  A score tile (128 rows x 128 keys, fp32) comes from
+//                   tensor memory into registers, its row maximum, exponentials and their sum are taken there, and the
+//                   probabilities go back as bf16 (the type of V, which the product needs);
+//   warps 8, 10:    issue tcgen05.mma: S = Q K^T from shared memory (8), O += P V with P from tensor memory (10);
+//   warp 9:         TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
+//   warp 11:        only completes the group of four whose registers the softmax warps take over (setmaxnreg).
 // Tensor memory: one score tile (128 columns), which the halves use in turn, the probabilities P of each half (64) and the
 // output O of each half (128), 512 in all.  A score tile is free as soon as its half has it in registers, so the tensor pipe
 // makes the next one, and the products with V, while the softmax runs: S0 | S1 | S0' P0 V | S1' P1 V | ...  Nothing goes
@@ -128,13 +127,12 @@ __device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------
 
 constexpr int kM = 128, kN = 128;              // rows of a half, keys of a block
-constexpr int kScoreWarp = 16, kTmaWarp = 17, kValueWarp = 18, kThreadsW = 640;
+constexpr int kScoreWarp = 8, kTmaWarp = 9, kValueWarp = 10, kThreadsW = 384;
 constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channel tile
-// Registers a thread: 640 x 96 at launch; a softmax thread holds 64 scores, the others need fewer.
-constexpr int kRegsSoft = 104, kRegsOther = 64;
-static_assert(512 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 96, "the groups' registers are those of the launch");
+// Registers a thread: 384 x 168 at launch; a softmax thread holds 128 scores, the others need fewer.
+constexpr int kRegsSoft = 208, kRegsOther = 88;
+static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
 constexpr unsigned kTmemS = 0, kTmemP = 128, kTmemO = 256, kTmemCols = 512;  // S, 2 x 64 of P, 2 x 128 of O
-constexpr int kPart = 64;                      // keys of a block that one of a row's two threads takes
 constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
 
 template <int DP>
@@ -148,11 +146,10 @@ template <int DP>
 struct __align__(1024) WindowSmem {
   unsigned char q[2][WindowCfg<DP>::kTileBytes];
   unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
-  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2], max_read[2];
+  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2];
   unsigned tmem_base;
   int poison[2];  // a value that is not finite lies in a block at the edge of the half's view
   int scan[kThreadsW / 32], found[6];
-  float row_max[2][2][kM];  // [half][thread of the row][row]: what the two threads of a row tell each other
 };
 
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned bar) {
@@ -374,10 +371,10 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.pv_done[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), 8), mbar_init(smem_u32(&sm.max_read[i]), 8);
+      mbar_init(smem_u32(&sm.p_full[i]), 4);
       sm.poison[i] = 0;
     }
-    mbar_init(smem_u32(&sm.s_free), 8);
+    mbar_init(smem_u32(&sm.s_free), 4);
     for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -502,27 +499,24 @@ __global__ void __launch_bounds__(kThreadsW, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
-    if ((warp >> 3) < halves) {
-      // ---- softmax of half h: thread (warp & 3) * 32 + lane of either group of four warps owns that row's 64 keys `sub` ----
-      const int h = warp >> 3, sub = (warp >> 2) & 1, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
-      const int rows_h = min(kM, t.rows - h * kM), in_half = (warp & 7) * 32 + lane;
+    if ((warp >> 2) < halves) {
+      // ---- softmax of half h: thread (warp & 3) * 32 + lane owns that row ----
+      const int h = warp >> 2, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
+      const int rows_h = min(kM, t.rows - h * kM);
       const unsigned lanes = unsigned((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + lanes + kTmemS + unsigned(sub) * kPart, tp = tmem + lanes + kTmemP + unsigned(h) * 64 + unsigned(sub) * 32;
-      const unsigned to = tmem + lanes + kTmemO + unsigned(h) * 128 + unsigned(sub) * (DP / 2);
+      const unsigned ts = tmem + lanes + kTmemS, tp = tmem + lanes + kTmemP + unsigned(h) * 64, to = tmem + lanes + kTmemO + unsigned(h) * 128;
       const Seen mine = seen_by(L, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
       // the first row of the half has the nearest end, the last row the farthest window start
       const Seen h_first = seen_by(L, rh0 + shift, t.nk), h_last = seen_by(L, rh0 + rows_h - 1 + shift, t.nk);
       const HalfView blocks = h == 0 ? view[0] : view[1];
-      auto meet = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + h) : "memory"); };  // the half's eight warps
-      float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), this thread's part of the sum
+      float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), sum
       int done = 0;                  // blocks that some row of the half sees, so far
       for (int j = 0; j < n_blocks; j++) {
         const int block = block_at(j);
         if (!blocks.has(block)) continue;
         const int key0 = block * kN;
         const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
-        // A wait that runs out does not leave the loop: the half's warps go on meeting, without waiting for anything else.
-        // The lanes of a warp agree on the outcome.
+        // A wait that runs out: the warp goes on without waiting for anything else.  Its lanes agree on the outcome.
         if (edge) {
           // V of this block, before the scores are there: zero what lies behind the sequence, look for values that are not
           // finite in the rest (an exponent of all ones carries into the sign bit when one is added to it)
@@ -533,62 +527,54 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           unsigned odd = 0;
           if (ok) {
 #pragma unroll
-            for (int i = 0; i < Cfg::kTileBytes / 16 / (2 * kM); i++) {
-              const uint4 x = vt[i * 2 * kM + in_half];
+            for (int i = 0; i < Cfg::kTileBytes / 16 / kM; i++) {
+              const uint4 x = vt[i * kM + row_h];
               constexpr unsigned e = 0x7f807f80u, one = 0x00800080u;
               const unsigned y = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
               // row of the tile: 8 chunks of 16 bytes a row, 128 rows of each 64 channels
-              if (((i * 2 * kM + in_half) >> 3) % kN < there) odd |= y;
+              if (((i * kM + row_h) >> 3) % kN < there) odd |= y;
             }
           }
           if (odd & 0x80008000u) sm.poison[h] = 1;
           if (ok && there < kN) {
-            for (int i = in_half; i < Cfg::kTileBytes / 16; i += 2 * kM)
+            for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM)
               if ((i >> 3) % kN >= there) vt[i] = make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
         ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(done) & 1u));
         fence_after();
-        unsigned s[2][32];
-        tmem_ld32(ts, s[0]);
-        tmem_ld32(ts + 32, s[1]);
+        unsigned s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, s[c]);
         tmem_wait_ld(s[0]);
-        tmem_touch(s[1]);
+        tmem_touch(s[1]), tmem_touch(s[2]), tmem_touch(s[3]);
         fence_before();
         __syncwarp();
         if (ok && lane == 0) mbar_arrive1(smem_u32(&sm.s_free));  // the other half's scores may come
         if (edge) {
           // bit i of below(n): i < n
           auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-          const int k0 = key0 + sub * kPart;
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const unsigned see = below(mine.first - k0 - 32 * c) | (below(mine.hi - k0 - 32 * c) & ~below(mine.lo - k0 - 32 * c));
+          for (int c = 0; c < 4; c++) {
+            const int k0 = key0 + 32 * c;
+            const unsigned see = below(mine.first - k0) | (below(mine.hi - k0) & ~below(mine.lo - k0));
 #pragma unroll
             for (int i = 0; i < 32; i++) s[c][i] = (see >> i) & 1u ? s[c][i] : 0xff800000u;
           }
         }
         float mx;
         {
-          float part[2];
+          float part[4];
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
+          for (int c = 0; c < 4; c++) {
             part[c] = max_nan(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]), __uint_as_float(s[c][2]));
 #pragma unroll
             for (int i = 3; i < 31; i += 2) part[c] = max_nan(part[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
           }
-          mx = max_nan(part[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
-          mx = max_nan(mx, part[1], part[1]);
+          mx = max_nan(max_nan(part[0], __uint_as_float(s[0][31]), part[1]), __uint_as_float(s[1][31]), max_nan(part[2], __uint_as_float(s[2][31]), part[3]));
+          mx = max_nan(mx, __uint_as_float(s[3][31]), mx);
         }
-        // The row's maximum is both threads'.  A slot is written again only when the last block's has been read.
-        if (done > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.max_read[h]), unsigned(done - 1) & 1u));
-        sm.row_max[h][sub][row_h] = mx;
-        meet();
-        const float other = sm.row_max[h][sub ^ 1][row_h];
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(smem_u32(&sm.max_read[h]));
-        mx = max_nan(mx, other, other);
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);  // a NaN or an infinity among the scores: the whole row is NaN
         const bool grow = (mx - m) * L.scale2 > kSlack;          // also the first finite score (m = -inf); false for NaN
         if (__any_sync(0xffffffffu, grow)) {
@@ -601,7 +587,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u));
             fence_after();
 #pragma unroll 1
-            for (int c = 0; c < DP / 32; c++) {
+            for (int c = 0; c < DP / 16; c++) {
               unsigned o[16];
               tmem_ld16(to + 16 * c, o);
 #pragma unroll
@@ -621,7 +607,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         };
         if (edge) {  // a masked score has to come out as exactly 0
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
+          for (int c = 0; c < 4; c++) {
             unsigned p[16];
             exp_chunk<false>(s[c], L.scale2, base, l4, p);
             if (c == 0) wait_p();
@@ -629,7 +615,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
+          for (int c = 0; c < 4; c++) {
             unsigned p[16];
             exp_chunk<true>(s[c], L.scale2, base, l4, p);
             if (c == 0) wait_p();
@@ -640,26 +626,23 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         done++;
       }
-      // ---- output: each of a row's two threads has half of the channels ----
+      // ---- output ----
       if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u);
       ok = __all_sync(0xffffffffu, ok);
-      sm.row_max[h][sub][row_h] = l;
-      meet();
-      l += sm.row_max[h][sub ^ 1][row_h];
       if (ok) {
         fence_after();
         const int64_t row = int64_t(t.q0) + rh0 + row_h;
         const bool on = row_h < rows_h;
         if (done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
-          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 7) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
-          for (int r = (warp & 7) * 16; r < min((warp & 7) * 16 + 16, rows_h); r++)
+          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 3) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
+          for (int r = (warp & 3) * 32; r < min((warp & 3) * 32 + 32, rows_h); r++)
             row_attention(L, int64_t(t.q0) + rh0 + r, head, t.k0, rh0 + r + shift, t.nk, qs);
         } else {
           const bool some = l > 0.f || l != l;
           const float f = some ? 1.f / l : 0.f;
-          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D + sub * (DP / 2);
+          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D;
 #pragma unroll 1
-          for (int c = 0; c < DP / 64; c++) {
+          for (int c = 0; c < DP / 32; c++) {
             unsigned o[32];
             if (done > 0) {
               tmem_ld32(to + 32 * c, o);
@@ -671,10 +654,10 @@ __global__ void __launch_bounds__(kThreadsW, 1)
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; e++) v[e] = some ? __uint_as_float(o[8 * i + e]) * f : 0.f;
-              if (sub * (DP / 2) + 32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
+              if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
             }
           }
-          if (on && sub == 0 && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
+          if (on && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
         }
       }
     }

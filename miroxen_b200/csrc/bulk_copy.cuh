@@ -47,12 +47,19 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
   }
   return false;
 }
-// The same without the sleeps, for hand-overs between warps that happen every microsecond or two: there the back-off of
-// mbar_wait would be longer than the wait itself.
-constexpr unsigned kSpinTries = 1u << 18;
+// The same without the sleeps and with the phase looked at first, for hand-overs between warps that happen every
+// microsecond or less and have mostly happened when they are waited for.
+constexpr unsigned kSpinTries = 1u << 22;
 __device__ __forceinline__ bool mbar_wait_spin(unsigned bar, unsigned parity) {
-  for (unsigned i = 0; i < kSpinTries; i++)
-    if (mbar_try(bar, parity)) return true;
+  for (unsigned i = 0; i < kSpinTries; i++) {
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
   return false;
 }
 // 1-D bulk copy global -> this CTA's shared memory; src, dst and bytes are multiples of 16.
