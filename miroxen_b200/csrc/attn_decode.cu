@@ -9,18 +9,21 @@
 // far from busy at this ratio, and the operands come from shared memory tiles that change with every use, which is
 // what the warp-level instruction takes without a detour.
 //
-// Split: a tile is kTile tokens of one (sequence, key head, block of 16 query heads).  All tiles of the call in order
+// Split: a tile is 64 or 128 tokens of one (sequence, key head, block of 16 query heads).  All tiles of the call in order
 // (sequence, head, token) are cut into equal runs, one per resident CTA, whatever the lengths are - a CTA's run may
 // end inside a sequence's tokens and cover several short sequences.  Each CTA finds the run's start itself by summing the
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
 // sum and unnormalised output in its slots of the workspace (one for the segment its run starts in, one for the segment
 // it ends in) and join_kernel, launched behind it, adds them up in order.  Results do not depend on timing.
 //
-// Within a CTA (4 warps): tiles of K and V come through a ring of shared-memory stages (16-byte cp.async, rows found
-// through the page table one tile ahead).  For the scores each warp takes kTile / 4 tokens; for the product with V each
-// warp takes D / 4 channels of all of them, so that the output stays in a few registers; maxima and probabilities pass
-// through shared memory.  Scores, maxima, sums and output are fp32; probabilities are rounded to bf16 (f16 for an e4m3
-// cache) for the product, as the tensor instruction needs the type of V.
+// Within a CTA a fifth warp brings the tiles of K and V into a ring of shared-memory stages (16-byte cp.async, rows found
+// through the page table one tile ahead, completion counted on mbarriers) and four warps do the arithmetic.  For the scores
+// each takes a quarter of the tile's tokens; for the product with V each takes a quarter of the channels of all tokens, so
+// that the output stays in a few registers and only the probabilities pass through shared memory.  They are taken relative
+// to a maximum that all four share and that moves only when a score lies more than 2^8 above it (every sum is relative to
+// it, so the result is the same): one barrier per tile, which also carries that vote.
+// Scores, maxima, sums and output are fp32; probabilities are rounded to bf16 (f16 for an e4m3 cache) for the product, as
+// the tensor instruction needs the type of V.
 #include <cuda_fp16.h>
 
 #include "bulk_copy.cuh"
@@ -31,10 +34,13 @@ namespace mxk {
 namespace {
 
 constexpr int kRows = 16;       // query heads per work item
-constexpr int kWarps = 4;
-constexpr int kThreadsD = 32 * kWarps;
-constexpr int kTile = 64;       // tokens per tile
-constexpr int kTokW = kTile / kWarps;
+constexpr int kWarps = 4;       // that compute; one more copies
+constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32;
+constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
+#ifndef MXK_TOKW
+#define MXK_TOKW(E, DP) 16
+#define MXK_STAGES(E, DP) ((E) || (DP) == 64 ? 4 : 3)
+#endif
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DecodeLaunch {
@@ -72,16 +78,24 @@ __device__ __forceinline__ View view_of(const DecodeLaunch& p, int b) {
 }
 
 // Tiles of sequence b, all its work items.
-__device__ __forceinline__ int tiles_of(const DecodeLaunch& p, int b) { return (view_of(p, b).len + kTile - 1) / kTile * p.heads; }
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const DecodeLaunch& p, int b) {
+  return (view_of(p, b).len + TILE - 1) / TILE * p.heads;
+}
 
 // Finds, with the whole CTA: the number of tiles of the call, and for tile `want` of the caller's choosing (a function of
 // the total) the sequence it lies in and the number of tiles in front of that sequence.
-template <class Want>
+template <int TILE, class Want>
 __device__ __forceinline__ void locate(const DecodeLaunch& p, int* red, Want want, int& total, int& seq, int& before) {
+  constexpr int W = kThreadsD / 32;
   const int n = p.c.n_seqs, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  int mine = 0;  // thread t sums a contiguous share of the sequences
+  int mine = 0, first = 0;  // thread t sums a contiguous share of the sequences
   const int share = (n + kThreadsD - 1) / kThreadsD, b0 = min(n, t * share), b1 = min(n, b0 + share);
-  for (int b = b0; b < b1; b++) mine += tiles_of(p, b);
+  for (int b = b0; b < b1; b++) {
+    const int k = tiles_of<TILE>(p, b);
+    if (b == b0) first = k;
+    mine += k;
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -89,12 +103,12 @@ __device__ __forceinline__ void locate(const DecodeLaunch& p, int* red, Want wan
     if (lane >= o) incl += x;
   }
   if (lane == 31) red[warp] = incl;
-  if (t == 0) red[kWarps] = -1;
+  if (t == 0) red[W] = -1;
   __syncthreads();
   int base = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; w++) {
+  for (int w = 0; w < W; w++) {
     if (w < warp) base += red[w];
     total += red[w];
   }
@@ -102,11 +116,11 @@ __device__ __forceinline__ void locate(const DecodeLaunch& p, int* red, Want wan
   const int target = want(total);
   if (target >= at && target < at + mine) {
     int b = b0;
-    for (int k = tiles_of(p, b); target >= at + k; k = tiles_of(p, b)) at += k, b++;
-    red[kWarps] = b, red[kWarps + 1] = at;
+    for (int k = first; target >= at + k; k = tiles_of<TILE>(p, b)) at += k, b++;
+    red[W] = b, red[W + 1] = at;
   }
   __syncthreads();
-  seq = red[kWarps], before = red[kWarps + 1];
+  seq = red[W], before = red[W + 1];
 }
 
 // A place in the order of tiles.
@@ -114,29 +128,42 @@ struct Cursor {
   int b, head, tile, n_tiles;  // tile of n_tiles of work item `head` (key head * blocks + block) of sequence b
   View v;
 };
+template <int TILE>
 __device__ __forceinline__ void cursor_sequence(const DecodeLaunch& p, Cursor& c) {  // sequences without a token are passed over
   while (c.b < p.c.n_seqs) {
     c.v = view_of(p, c.b);
-    c.n_tiles = (c.v.len + kTile - 1) / kTile;
+    c.n_tiles = (c.v.len + TILE - 1) / TILE;
     if (c.n_tiles > 0) return;
     c.b++;
   }
 }
+template <int TILE>
 __device__ __forceinline__ void cursor_next(const DecodeLaunch& p, Cursor& c) {
   if (++c.tile < c.n_tiles) return;
   c.tile = 0;
   if (++c.head < p.heads) return;
   c.head = 0, c.b++;
-  cursor_sequence(p, c);
+  cursor_sequence<TILE>(p, c);
 }
 
-__device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes, or 16 zeros
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, unsigned bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One arrival on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(unsigned bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Barrier of the computing warps; `vote`: whether any of them has v set.
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
+__device__ __forceinline__ bool vote(bool v) {
+  unsigned r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, 1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(r)
+               : "r"(unsigned(v)), "n"(kConsumers)
+               : "memory");
+  return r != 0;
 }
 __device__ __forceinline__ void ldsm4(unsigned addr, unsigned (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -166,22 +193,18 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 
-// Shared-memory layout of a stage: rows of DP elements, one per token, in 16-byte chunks; chunk j of row t sits at
-// chunk position chunk_at(t, j), which keeps the eight rows an ldmatrix phase (or the two rows a 128-bit load phase of
-// the e4m3 keys) reads off each other's banks.
-template <bool E4M3, int DP, bool IS_V>
-__device__ __forceinline__ int chunk_at(int t, int j) {
-  if (!E4M3) return j ^ (t & 7);                                      // rows of 256 or 128 bytes
-  if (DP == 128) return IS_V ? j ^ (t & 7) : j ^ ((t & 1) << 2);      // rows of 128 bytes
-  return IS_V ? j ^ ((t >> 1) & 3) : j;                               // rows of 64 bytes
-}
-
+// A stage holds a tile of K and one of V, a row per token, rows 16 bytes longer than their DP elements: the eight rows that
+// an ldmatrix phase reads then start four banks apart.  Tokens per tile and stages: about 32 KB a stage where a token's row
+// is long, twice the tokens where it is short, so that what a tile costs beside its bytes (a barrier, the vote, the
+// exchange of probabilities) is spread over as many.
 template <bool E4M3, int DP>
 struct DecodeCfg {
-  static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2);
+  static constexpr int kTokW = MXK_TOKW(E4M3, DP);  // tokens per warp
+  static constexpr int kTile = kTokW * kWarps;
+  static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2), kPitch = kRowBytes + 16;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kTileBytes = kTile * kRowBytes;
-  static constexpr int kStages = E4M3 || DP == 64 ? 4 : 3;
+  static constexpr int kTileBytes = kTile * kPitch;
+  static constexpr int kStages = MXK_STAGES(E4M3, DP);
   static constexpr int kSmem = kStages * 2 * kTileBytes;
 };
 
@@ -189,25 +212,32 @@ template <bool E4M3, int DP>
 __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant__ DecodeLaunch p) {
   using Cfg = DecodeCfg<E4M3, DP>;
   using elem = typename KvElem<E4M3>::type;
-  constexpr int kSt = Cfg::kStages, kKSteps = DP / 16, kNW = DP / kWarps / 8;  // k-steps of the scores; 8-channel tiles per warp
+  constexpr int kSt = Cfg::kStages, kTile = Cfg::kTile, kTokW = Cfg::kTokW, kPitch = Cfg::kPitch;
+  constexpr int kKSteps = DP / 16, kNW = DP / kWarps / 8, kNT = kTokW / 8;  // k-steps of the scores; 8-channel tiles, 8-token tiles per warp
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ int64_t offs[kSt + 1][kTile];  // element offset of each token of a tile (its head included), -1: not there
+  __shared__ __align__(16) unsigned short prob[2][kRows][kTile + 8];
   __shared__ float wmax[kWarps][kRows], wsum[kWarps][kRows];
-  __shared__ __align__(16) unsigned short prob[kRows][kTile + 8];
-  __shared__ int red[kWarps + 2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int D = p.c.D, chunks = D * int(sizeof(elem)) / 16;
+  __shared__ unsigned there[kSt][kTile / 32];  // which tokens of a tile exist
+  __shared__ unsigned long long full[kSt], empty[kSt];
+  __shared__ int red[kThreadsD / 32 + 2];
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int D = p.c.D;
+  const unsigned ring_u = smem_u32(ring);
   pdl_launch_dependents();
-  // channels [D, DP) of every row stay zero (the copies never touch them)
-  if (D < DP) {
+  if (tid == 0) {
+    // a stage is full when the copies of the copying warp's 32 threads have landed and its word on the tokens is written
+    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&full[i]), 33), mbar_init(smem_u32(&empty[i]), kWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (D < DP) {  // channels [D, DP) of every row stay zero (the copies never touch them)
     for (int i = tid; i < Cfg::kSmem / 16; i += kThreadsD) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   pdl_wait();
 
   int total, seq0, before;
   int per = 0;
-  locate(p, red, [&](int t) { return int(blockIdx.x) * (per = (t + p.ctas - 1) / p.ctas); }, total, seq0, before);
-  const int t0 = min(total, int(blockIdx.x) * per), t1 = min(total, t0 + per);
+  locate<kTile>(p, red, [&](int t) { return int(blockIdx.x) * (per = (t + p.ctas - 1) / p.ctas); }, total, seq0, before);
+  const int t0 = min(total, int(blockIdx.x) * per), n_my = min(total, t0 + per) - t0;
   // sequences that have no token in view: out 0, lse -inf
   for (int b = blockIdx.x; b < p.c.n_seqs; b += gridDim.x) {
     if (view_of(p, b).len > 0) continue;
@@ -215,85 +245,91 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     if (p.a.lse)
       for (int i = tid; i < p.a.H; i += kThreadsD) p.a.lse[int64_t(b) * p.a.H + i] = -INFINITY;
   }
-  if (t0 >= t1) return;
+  if (n_my <= 0) return;
 
-  Cursor cur;  // of the arithmetic
+  Cursor cur;
   cur.b = seq0;
-  cursor_sequence(p, cur);
+  cursor_sequence<kTile>(p, cur);
   cur.head = (t0 - before) / cur.n_tiles, cur.tile = (t0 - before) % cur.n_tiles;
-  Cursor look = cur;  // of the page look-ups, kSt tiles ahead
-  const int n_my = t1 - t0;
-  int looked = 0;
-  // the page look-up of one tile: thread t the tile's token t
-  auto look_up = [&]() -> int64_t {
-    int64_t off = -1;
-    if (looked < n_my) {
-      if (tid < kTile) {
-        const int i = look.tile * kTile + tid;
-        if (i < look.v.len) {
-          const int tok = i < look.v.first ? i : i - look.v.first + look.v.skip;
-          off = kv_token_offset(p.c, look.b, tok);
-          if (off < 0) {
-            if (p.err) atomicExch(p.err, kErrBadIndex);
-          } else {
-            off += int64_t(look.head / p.blocks) * p.c.head_stride;
+  bool ok = true;
+
+  if (warp == kWarps) {
+    // ---- the copying warp ----
+    constexpr int kPerInstr = 32 / Cfg::kChunks, kWords = kTile / 32;  // rows per instruction; tokens a lane looks up
+    const int ch = lane % Cfg::kChunks, sub = lane / Cfg::kChunks;
+    const bool copies = ch * 16 < D * int(sizeof(elem));
+    const unsigned char *kb = static_cast<const unsigned char*>(p.c.k) + ch * 16, *vb = static_cast<const unsigned char*>(p.c.v) + ch * 16;
+    int64_t off[kWords];  // byte offsets of tokens lane, lane + 32, ... of the tile that is copied next, -1: not there
+    auto look_up = [&]() {
+      const int64_t head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
+#pragma unroll
+      for (int u = 0; u < kWords; u++) {
+        const int i = cur.tile * kTile + u * 32 + lane;
+        off[u] = -1;
+        if (i < cur.v.len) {
+          off[u] = kv_token_offset(p.c, cur.b, i < cur.v.first ? i : i - cur.v.first + cur.v.skip);
+          if (off[u] >= 0) off[u] = (off[u] + head_off) * int(sizeof(elem));
+          else if (p.err) atomicExch(p.err, kErrBadIndex);
+        }
+      }
+      cursor_next<kTile>(p, cur);
+    };
+    look_up();
+    int st = 0;
+    for (int i = 0; i < n_my; i++) {
+      if (i >= kSt) {
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u));
+        if (!ok) break;
+      }
+      const unsigned dk = ring_u + unsigned(st) * 2 * Cfg::kTileBytes + unsigned(sub * kPitch + ch * 16);
+#pragma unroll
+      for (int u = 0; u < kWords; u++) {
+        const unsigned word = __ballot_sync(0xffffffffu, off[u] >= 0);
+        if (lane == 0) there[st][u] = word;
+#pragma unroll
+        for (int r = 0; r < 32 / kPerInstr; r++) {
+          const int row = u * 32 + r * kPerInstr;  // + sub
+          const int64_t o = __shfl_sync(0xffffffffu, off[u], r * kPerInstr + sub);
+          if (copies) {  // a token that is not there reads as zeros: its value must not carry anything into 0 * v
+            const unsigned n = o >= 0 ? 16u : 0u;
+            const int64_t x = o >= 0 ? o : 0;
+            cp_async16(dk + unsigned(row * kPitch), kb + x, n);
+            cp_async16(dk + unsigned(Cfg::kTileBytes + row * kPitch), vb + x, n);
           }
         }
       }
-      cursor_next(p, look);
+      cp_async_arrive(smem_u32(&full[st]));
+      if (lane == 0) arrive(smem_u32(&full[st]));
+      if (i + 1 < n_my) look_up();  // the page table's latency passes while this tile is on its way
+      if (++st == kSt) st = 0;
     }
-    looked++;
-    return off;
-  };
-  const unsigned ring_u = smem_u32(ring);
-  auto copy_tile = [&](int i) {  // tile i of the run into its stage
-    if (i < n_my) {
-      const unsigned st = ring_u + unsigned(i % kSt) * 2 * Cfg::kTileBytes;
-      const int64_t* of = offs[i % (kSt + 1)];
-      for (int j = tid; j < kTile * chunks; j += kThreadsD) {
-        const int t = D == DP ? j / Cfg::kChunks : j / chunks, ch = D == DP ? j % Cfg::kChunks : j - t * chunks;
-        const int64_t off = of[t];
-        const unsigned dk = st + unsigned(t * Cfg::kRowBytes + chunk_at<E4M3, DP, false>(t, ch) * 16);
-        const unsigned dv = st + Cfg::kTileBytes + unsigned(t * Cfg::kRowBytes + chunk_at<E4M3, DP, true>(t, ch) * 16);
-        if (off >= 0) {
-          cp_async16(dk, static_cast<const elem*>(p.c.k) + off + ch * (16 / int(sizeof(elem))));
-          cp_async16(dv, static_cast<const elem*>(p.c.v) + off + ch * (16 / int(sizeof(elem))));
-        } else {  // a token that is not there: its value must not carry anything into 0 * v
-          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(ring + (dk - ring_u)) = z;
-          *reinterpret_cast<uint4*>(ring + (dv - ring_u)) = z;
-        }
-      }
-    }
-    cp_commit();
-  };
-  for (int i = 0; i < kSt; i++) {
-    const int64_t off = look_up();
-    if (tid < kTile) offs[i][tid] = off;
+    // nothing of this CTA's may be under way when its shared memory goes
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok && p.err) atomicExch(p.err, kErrBulkTimeout);
+    return;
   }
-  __syncthreads();
-  for (int i = 0; i < kSt - 1; i++) copy_tile(i);
 
-  // this warp's state: rows r0 = lane / 4 and r0 + 8; channel tile n of the warp: channels (warp * kNW + n) * 8 ..
-  // (e4m3: see the product with V) of the output
+  // ---- the computing warps ----
+  // this warp's state: rows r0 = lane / 4 and r0 + 8; channel tiles of the warp's quarter of the output
   float o[kNW][4];
-  float m[2], l[2];
+  float base[2], l[2];  // maximum in use (in units of log2), this thread's part of the sum
   unsigned qf[kKSteps][4];
-  float qs[2] = {1.f, 1.f};
+  float qs[2] = {1.f, 1.f}, ks2 = 0.f;
   const int r0 = lane >> 2, c2 = (lane & 3) * 2;
   bool fresh = true;
-  int first_tile = cur.tile;
+  int first_tile = 0, st = 0, g = 0, rows = 0, h0 = 0;
+  unsigned ph = 0;
 
   for (int i = 0; i < n_my; i++) {
-    const int64_t next_off = look_up();  // of tile i + kSt; the page table's latency passes during this tile
-    const int g = cur.head / p.blocks, blk = cur.head % p.blocks;
-    const int rows = min(kRows, p.group - blk * kRows);
-    const int h0 = g * p.group + blk * kRows;
     if (fresh) {  // a new (sequence, head): its queries into registers
       fresh = false, first_tile = cur.tile;
+      g = cur.head / p.blocks;
+      const int blk = cur.head - g * p.blocks;
+      rows = min(kRows, p.group - blk * kRows), h0 = g * p.group + blk * kRows;
+      ks2 = p.scale2 * (E4M3 && p.c.k_scale ? p.c.k_scale[g] : 1.f);
 #pragma unroll
       for (int n = 0; n < kNW; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
+      base[0] = base[1] = -INFINITY, l[0] = l[1] = 0.f;
       const mxk_bf16* q = p.a.q + int64_t(cur.b) * p.a.q_stride + int64_t(h0) * D;
 #pragma unroll
       for (int half = 0; half < 2; half++) {
@@ -310,14 +346,14 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         } else {
           // e4m3 keys are taken as f16, which holds them exactly; so are the queries, scaled by a power of two (per head)
           // that brings their largest into [2^13, 2^14): what f16 then loses lies 2^-38 below it.  The order of channels in
-          // a 64-channel group is the one the keys are read in: step s, lane c: channels 16 c + 4 s + {0, 1 | 2, 3}.
+          // a 16-channel step is the one the keys are read in: lane c: channels 4 c + {0, 1 | 2, 3}.
           unsigned raw[kKSteps][2];
           float big = 0.f;
 #pragma unroll
           for (int s = 0; s < kKSteps; s++)
 #pragma unroll
             for (int hi = 0; hi < 2; hi++) {
-              const int d = 64 * (s / 4) + 8 * c2 + 4 * (s % 4) + 2 * hi;
+              const int d = 16 * s + 2 * c2 + 2 * hi;
               raw[s][hi] = on && d < D ? *reinterpret_cast<const unsigned*>(q + int64_t(r) * D + d) : 0u;
               big = fmaxf(big, fmaxf(fabsf(bf16_lo(raw[s][hi])), fabsf(bf16_hi(raw[s][hi]))));
             }
@@ -335,90 +371,108 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         }
       }
     }
-    cp_wait<kSt - 2>();
-    __syncthreads();  // tile i has landed for everyone, and nobody still reads the stage that is filled next
-    copy_tile(i + kSt - 1);
+    // A wait that runs out does not leave the loop: the four warps go on meeting, without waiting for anything else.
+    ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&full[st]), ph));
+    const unsigned k_u = ring_u + unsigned(st) * 2 * Cfg::kTileBytes, v_u = k_u + Cfg::kTileBytes;
 
-    // ---- scores of this warp's 16 tokens ----
-    const unsigned char* kt = ring + (i % kSt) * 2 * Cfg::kTileBytes;
-    const unsigned k_u = ring_u + unsigned(i % kSt) * 2 * Cfg::kTileBytes, v_u = k_u + Cfg::kTileBytes;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // ---- scores of this warp's tokens ----
+    float s[kNT][4];
+#pragma unroll
+    for (int n = 0; n < kNT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
     if (!E4M3) {
-      const int t = warp * kTokW + (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
 #pragma unroll
-      for (int ks = 0; ks < kKSteps; ks++) {
-        unsigned b[4];
-        ldsm4(k_u + unsigned(t * Cfg::kRowBytes + chunk_at<E4M3, DP, false>(t, 2 * ks + hi) * 16), b);
-        mma16816<false>(s[0], qf[ks], b[0], b[1]);
-        mma16816<false>(s[1], qf[ks], b[2], b[3]);
-      }
+      for (int ks = 0; ks < kKSteps; ks++)
+#pragma unroll
+        for (int n = 0; n < kNT; n += 2) {
+          unsigned b[4];
+          ldsm4(a + unsigned(n * 8 * kPitch + ks * 32), b);
+          mma16816<false>(s[n], qf[ks], b[0], b[1]);
+          mma16816<false>(s[n + 1], qf[ks], b[2], b[3]);
+        }
     } else {
+      // four 16-byte chunks of 8 tokens: a register holds four channels of one token, two pairs of one 16-channel step
+      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 7)) * kPitch + (lane >> 3) * 16);
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const int t = warp * kTokW + 8 * n + r0;
+      for (int grp = 0; grp < DP / 64; grp++)
 #pragma unroll
-        for (int grp = 0; grp < DP / 64; grp++) {
-          const uint4 kv = *reinterpret_cast<const uint4*>(kt + t * Cfg::kRowBytes + chunk_at<E4M3, DP, false>(t, 4 * grp + (lane & 3)) * 16);
-          const unsigned w[4] = {kv.x, kv.y, kv.z, kv.w};
+        for (int n = 0; n < kNT; n++) {
+          unsigned w[4];
+          ldsm4(a + unsigned(n * 8 * kPitch + grp * 64), w);
 #pragma unroll
           for (int ks = 0; ks < 4; ks++) mma16816<true>(s[n], qf[4 * grp + ks], e4m3x2_to_f16x2(w[ks] & 0xffffu), e4m3x2_to_f16x2(w[ks] >> 16));
         }
-      }
     }
-    const float ks2 = p.scale2 * (E4M3 && p.c.k_scale ? p.c.k_scale[g] : 1.f);
-    const int64_t* of = offs[i % (kSt + 1)] + warp * kTokW;
-    float mx[2] = {-INFINITY, -INFINITY};
+    // the warp's bits of the tile's tokens
+    const unsigned word = there[st][warp * kTokW / 32] >> (warp * kTokW % 32);
+    const bool all_there = kTokW == 32 ? word == 0xffffffffu : (word & 0xffffu) == 0xffffu;
+    const float f0 = E4M3 ? ks2 * qs[0] : ks2, f1 = E4M3 ? ks2 * qs[1] : ks2;
 #pragma unroll
-    for (int n = 0; n < 2; n++)
+    for (int n = 0; n < kNT; n++) s[n][0] *= f0, s[n][1] *= f0, s[n][2] *= f1, s[n][3] *= f1;
+    if (!all_there) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const bool there = of[8 * n + c2 + (e & 1)] >= 0;
-        s[n][e] = there ? s[n][e] * (E4M3 ? ks2 * qs[e >> 1] : ks2) : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      }
+      for (int n = 0; n < kNT; n++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      if ((lane & 3) == 0) wmax[warp][r0 + 8 * h] = mx[h];
+        for (int e = 0; e < 4; e++)
+          if (!(word >> (8 * n + c2 + (e & 1)) & 1u)) s[n][e] = -INFINITY;
     }
-    __syncthreads();
-    if (tid < kTile) offs[(i + kSt) % (kSt + 1)][tid] = next_off;  // the slot of tile i - 1
-    float base[2];
+    float mx[2] = {fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])};
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float mn = m[h];
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) mn = fmaxf(mn, wmax[w][r0 + 8 * h]);
-      base[h] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: exp2(-inf - 0) = 0 everywhere
-      if (mn != m[h]) {
-        const float f = ex2_approx(m[h] - base[h]);  // 0 for the first maximum
-        l[h] *= f;
-#pragma unroll
-        for (int n = 0; n < kNW; n++) o[n][2 * h] *= f, o[n][2 * h + 1] *= f;
-        m[h] = mn;
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < 2; n++)
+    for (int n = 1; n < kNT; n++) mx[0] = fmaxf(mx[0], fmaxf(s[n][0], s[n][1])), mx[1] = fmaxf(mx[1], fmaxf(s[n][2], s[n][3]));
+    unsigned short(*pr)[kTile + 8] = prob[i & 1];
+    float add[2];
+    auto probabilities = [&]() {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float p0 = ex2_approx(s[n][2 * h] - base[h]), p1 = ex2_approx(s[n][2 * h + 1] - base[h]);
-        l[h] += p0 + p1;
-        *reinterpret_cast<unsigned*>(&prob[r0 + 8 * h][warp * kTokW + 8 * n + c2]) = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+        const float b = base[h] == -INFINITY ? 0.f : base[h];  // nothing seen yet: exp2(-inf - 0) = 0 everywhere
+        add[h] = 0.f;
+#pragma unroll
+        for (int n = 0; n < kNT; n++) {
+          const float p0 = ex2_approx(s[n][2 * h] - b), p1 = ex2_approx(s[n][2 * h + 1] - b);
+          add[h] += p0 + p1;
+          *reinterpret_cast<unsigned*>(&pr[r0 + 8 * h][warp * kTokW + 8 * n + c2]) = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+        }
       }
-    __syncthreads();
+    };
+    probabilities();
+    if (vote(mx[0] > base[0] + kSlack || mx[1] > base[1] + kSlack)) {  // always in a segment's first tile
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        if ((lane & 3) == 0) wmax[warp][r0 + 8 * h] = mx[h];
+      }
+      meet();
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float mn = base[h];
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) mn = fmaxf(mn, wmax[w][r0 + 8 * h]);
+        if (mn != base[h]) {
+          const float f = ex2_approx(base[h] - mn);  // 0 for the first maximum
+          l[h] *= f;
+#pragma unroll
+          for (int n = 0; n < kNW; n++) o[n][2 * h] *= f, o[n][2 * h + 1] *= f;
+          base[h] = mn;
+        }
+      }
+      probabilities();
+      meet();
+    }
+    l[0] += add[0], l[1] += add[1];
     // ---- this warp's channels of the product with V ----
+    const unsigned pa_u = smem_u32(&pr[(lane & 7) + (((lane >> 3) & 1) << 3)][(lane >> 4) << 3]);
+    const unsigned va_u = v_u + unsigned(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch) +
+                          unsigned((E4M3 ? (kNW / 2 == 2 ? warp * 2 + (lane >> 4) : warp) : warp * kNW + (lane >> 4)) * 16);
 #pragma unroll
     for (int ks = 0; ks < kTile / 16; ks++) {
       unsigned pa[4];
-      ldsm4(smem_u32(&prob[(lane & 7) + (((lane >> 3) & 1) << 3)][16 * ks + ((lane >> 4) << 3)]), pa);
-      const int t = 16 * ks + (lane & 7) + (((lane >> 3) & 1) << 3);
+      ldsm4(pa_u + unsigned(ks * 32), pa);
       if (!E4M3) {
 #pragma unroll
         for (int n = 0; n < kNW; n += 2) {
           unsigned b[4];
-          ldsm4_t(v_u + unsigned(t * Cfg::kRowBytes + chunk_at<E4M3, DP, true>(t, warp * kNW + n + (lane >> 4)) * 16), b);
+          ldsm4_t(va_u + unsigned(ks * 16 * kPitch + n * 16), b);
           mma16816<false>(o[n], pa, b[0], b[1]);
           mma16816<false>(o[n + 1], pa, b[2], b[3]);
         }
@@ -427,8 +481,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         // the pairs of one channel are then its bytes 0, 2 and 1, 3, so two channel tiles hold the even and the odd ones
         constexpr int kPairs = kNW / 2;  // 16-byte chunks of the warp (16 channels each)
         unsigned b[4];
-        const int ch = kPairs == 2 ? warp * 2 + (lane >> 4) : warp;
-        ldsm4_t(v_u + unsigned(t * Cfg::kRowBytes + chunk_at<E4M3, DP, true>(t, ch) * 16), b);
+        ldsm4_t(va_u + unsigned(ks * 16 * kPitch), b);
 #pragma unroll
         for (int n = 0; n < kPairs; n++) {
           const unsigned lo = b[2 * n], hi = b[2 * n + 1];  // tokens 0-7 and 8-15 of the step
@@ -437,6 +490,9 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         }
       }
     }
+    __syncwarp();
+    if (lane == 0) arrive(smem_u32(&empty[st]));
+    if (++st == kSt) st = 0, ph ^= 1u;
 
     const bool last = cur.tile + 1 == cur.n_tiles;
     if (last || i + 1 == n_my) {  // the (sequence, head) or the run ends: store
@@ -447,7 +503,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         if ((lane & 3) == 0) wsum[warp][r0 + 8 * h] = l[h];
       }
-      __syncthreads();
+      meet();
       const float vs = E4M3 && p.c.v_scale ? p.c.v_scale[g] : 1.f;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -474,34 +530,34 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         }
         if (warp == 0 && (lane & 3) == 0) {
           if (!whole) {
-            p.part_ml[(slot * kRows + r) * 2] = m[h], p.part_ml[(slot * kRows + r) * 2 + 1] = sum;
+            p.part_ml[(slot * kRows + r) * 2] = base[h], p.part_ml[(slot * kRows + r) * 2 + 1] = sum;
           } else if (p.a.lse) {
-            p.a.lse[int64_t(cur.b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (m[h] + log2f(sum)) * kLn2;
+            p.a.lse[int64_t(cur.b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (base[h] + log2f(sum)) * kLn2;
           }
         }
       }
       fresh = true;
     }
-    cursor_next(p, cur);
+    cursor_next<kTile>(p, cur);
   }
-  cp_wait<0>();
+  if (!ok && p.err) atomicExch(p.err, kErrBulkTimeout);
 }
 
 // Adds up, for each (sequence, head) that several runs share, the parts in the order of the runs.
-template <int DP>
-__global__ void __launch_bounds__(kThreadsD) join_kernel(const __grid_constant__ DecodeLaunch p) {
+template <int DP, int TILE>
+__global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant__ DecodeLaunch p) {
   __shared__ int red[kWarps + 2];
   pdl_launch_dependents();
   pdl_wait();
   const int b = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - b * p.heads;
-  const int n_tiles = (view_of(p, b).len + kTile - 1) / kTile;
+  const int n_tiles = (view_of(p, b).len + TILE - 1) / TILE;
   // tiles in front of sequence b and in total
   int total = 0, before = 0;
   {
     const int n = p.c.n_seqs, t = threadIdx.x;
     int all = 0, front = 0;
-    for (int x = t; x < n; x += kThreadsD) {
-      const int k = tiles_of(p, x);
+    for (int x = t; x < n; x += kConsumers) {
+      const int k = tiles_of<TILE>(p, x);
       all += k;
       if (x < b) front += k;
     }
@@ -520,7 +576,7 @@ __global__ void __launch_bounds__(kThreadsD) join_kernel(const __grid_constant__
   const int rows = min(kRows, p.group - blk * kRows), h0 = g * p.group + blk * kRows, D = p.c.D;
   // slot of run c: the segment it starts in, unless the segment starts inside the run (or with it)
   auto slot = [&](int c) { return 2 * int64_t(c) + (c == c0 ? 1 : 0); };
-  for (int i = threadIdx.x; i < rows * D; i += kThreadsD) {
+  for (int i = threadIdx.x; i < rows * D; i += kConsumers) {
     const int r = i / D, d = i - r * D;
     float mx = -INFINITY;
     for (int c = c0; c <= c1; c++) mx = fmaxf(mx, p.part_ml[(slot(c) * kRows + r) * 2]);
@@ -549,13 +605,13 @@ template <bool E4M3, int DP>
 int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   p.ctas = decode_ctas<E4M3, DP>();
   // no more runs than there can be tiles
-  const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, kTile);
+  const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, DecodeCfg<E4M3, DP>::kTile);
   if (p.ctas > most) p.ctas = int(most < 1 ? 1 : most);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
   launch_pdl(decode_kernel<E4M3, DP>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
   if (int rc = after_launch(name)) return rc;
-  launch_pdl(join_kernel<DP>, dim3(unsigned(p.c.n_seqs * p.heads)), dim3(kThreadsD), 0, s, p);
+  launch_pdl(join_kernel<DP, DecodeCfg<E4M3, DP>::kTile>, dim3(unsigned(p.c.n_seqs * p.heads)), dim3(kConsumers), 0, s, p);
   return after_launch(name);
 }
 
@@ -602,7 +658,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   p.group = a.H / cache->Hkv;
   p.blocks = int(ceil_div(p.group, kRows));
   p.heads = cache->Hkv * p.blocks;
-  const int64_t tiles = int64_t(cache->n_seqs) * p.heads * (ceil_div(int64_t(cache->max_pages) * cache->page_size, kTile) + 1);
+  const int64_t tiles = int64_t(cache->n_seqs) * p.heads * (ceil_div(int64_t(cache->max_pages) * cache->page_size, 64) + 1);
   if (tiles >= (int64_t(1) << 30)) return fail(MXK_ERR_TOO_LARGE, "%s: n_seqs * heads * tokens too large (%lld tiles)", name, (long long)tiles);
   p.scale2 = a.scale * kLog2e;
   p.err = device_error_word();
