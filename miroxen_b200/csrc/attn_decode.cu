@@ -51,6 +51,7 @@ struct DecodeLaunch {
   int heads;       // Hkv * blocks: work items per sequence
   int ctas;        // runs
   float scale2;    // scale * log2(e)
+  unsigned page_recip;  // floor((2^32 - 1) / page_size)
   float* part_o;   // [2 ctas][16][DP]
   float* part_ml;  // [2 ctas][16][2]
   int* err;
@@ -259,17 +260,23 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     const int ch = lane % Cfg::kChunks, sub = lane / Cfg::kChunks;
     const bool copies = ch * 16 < D * int(sizeof(elem));
     const unsigned char *kb = static_cast<const unsigned char*>(p.c.k) + ch * 16, *vb = static_cast<const unsigned char*>(p.c.v) + ch * 16;
-    int64_t off[kWords];  // byte offsets of tokens lane, lane + 32, ... of the tile that is copied next, -1: not there
+    // Pages and slots of tokens lane, lane + 32, ... of the tile that is copied next (slot -1: no token), asked for before the
+    // tile in front of it is copied and not looked at until then, so that the page table's latency passes meanwhile.
+    int page[kWords], slot[kWords];
+    int64_t head_off;
     auto look_up = [&]() {
-      const int64_t head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
+      head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
 #pragma unroll
       for (int u = 0; u < kWords; u++) {
         const int i = cur.tile * kTile + u * 32 + lane;
-        off[u] = -1;
-        if (i < cur.v.len) {
-          off[u] = kv_token_offset(p.c, cur.b, i < cur.v.first ? i : i - cur.v.first + cur.v.skip);
-          if (off[u] >= 0) off[u] = (off[u] + head_off) * int(sizeof(elem));
-          else if (p.err) atomicExch(p.err, kErrBadIndex);
+        page[u] = 0, slot[u] = -1;
+        if (i < cur.v.len) {  // inside the table: the length is held to it
+          const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
+          // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
+          int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
+          if (r >= p.c.page_size) n++, r -= p.c.page_size;
+          slot[u] = r;
+          page[u] = p.c.page_table[int64_t(cur.b) * p.c.table_stride + n];
         }
       }
       cursor_next<kTile>(p, cur);
@@ -277,6 +284,16 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     look_up();
     int st = 0;
     for (int i = 0; i < n_my; i++) {
+      int64_t off[kWords];  // byte offsets, -1: not there
+#pragma unroll
+      for (int u = 0; u < kWords; u++) {
+        off[u] = -1;
+        if (slot[u] >= 0) {
+          if (page[u] >= 0 && page[u] < p.c.num_pages) off[u] = (int64_t(page[u]) * p.c.page_stride + int64_t(slot[u]) * p.c.token_stride + head_off) * int(sizeof(elem));
+          else if (p.err) atomicExch(p.err, kErrBadIndex);
+        }
+      }
+      if (i + 1 < n_my) look_up();
       if (i >= kSt) {
         ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u));
         if (!ok) break;
@@ -300,7 +317,6 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       }
       cp_async_arrive(smem_u32(&full[st]));
       if (lane == 0) arrive(smem_u32(&full[st]));
-      if (i + 1 < n_my) look_up();  // the page table's latency passes while this tile is on its way
       if (++st == kSt) st = 0;
     }
     // nothing of this CTA's may be under way when its shared memory goes
@@ -661,6 +677,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   const int64_t tiles = int64_t(cache->n_seqs) * p.heads * (ceil_div(int64_t(cache->max_pages) * cache->page_size, 64) + 1);
   if (tiles >= (int64_t(1) << 30)) return fail(MXK_ERR_TOO_LARGE, "%s: n_seqs * heads * tokens too large (%lld tiles)", name, (long long)tiles);
   p.scale2 = a.scale * kLog2e;
+  p.page_recip = 0xffffffffu / unsigned(cache->page_size);
   p.err = device_error_word();
   const cudaStream_t s = as_stream(stream);
   if (cache->D <= 64) return cache->type == MXK_KV_E4M3 ? launch_decode<true, 64>(name, p, s) : launch_decode<false, 64>(name, p, s);
