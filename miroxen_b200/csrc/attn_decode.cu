@@ -559,55 +559,76 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   if (!ok && p.err) atomicExch(p.err, kErrBulkTimeout);
 }
 
-// Adds up, for each (sequence, head) that several runs share, the parts in the order of the runs.
+// Adds up, for each (sequence, head) that several runs share, the parts in the order of the runs: one CTA per work item and
+// row, warp w taking parts w, w + 4, ... (all channels of a part per access, several parts in flight), the warps' sums in
+// order at the end.
 template <int DP, int TILE>
 __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant__ DecodeLaunch p) {
-  __shared__ int red[kWarps + 2];
+  constexpr int kCh = DP / 32;  // channels of a lane
+  __shared__ int sums[2][kWarps];
+  __shared__ float top[kWarps], part_l[kWarps], part[kWarps][DP];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - b * p.heads;
-  const int n_tiles = (view_of(p, b).len + TILE - 1) / TILE;
-  // tiles in front of sequence b and in total
+  const int b = int(blockIdx.x) / p.heads, head = int(blockIdx.x) - b * p.heads, r = int(blockIdx.y);
+  const int g = head / p.blocks, blk = head - g * p.blocks, h = g * p.group + blk * kRows + r;
+  if (r >= min(kRows, p.group - blk * kRows)) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // tiles in total and in front of sequence b
   int total = 0, before = 0;
-  {
-    const int n = p.c.n_seqs, t = threadIdx.x;
-    int all = 0, front = 0;
-    for (int x = t; x < n; x += kConsumers) {
-      const int k = tiles_of<TILE>(p, x);
-      all += k;
-      if (x < b) front += k;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), front += __shfl_xor_sync(0xffffffffu, front, o);
-    __shared__ int fr[kWarps];
-    if ((t & 31) == 0) red[t >> 5] = all, fr[t >> 5] = front;
-    __syncthreads();
-    for (int w = 0; w < kWarps; w++) total += red[w], before += fr[w];
+  for (int x = tid; x < p.c.n_seqs; x += kConsumers) {
+    const int k = tiles_of<TILE>(p, x);
+    total += k;
+    if (x < b) before += k;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) sums[0][warp] = total, sums[1][warp] = before;
+  __syncthreads();
+  total = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3], before = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  const int n_tiles = (view_of(p, b).len + TILE - 1) / TILE;
   if (n_tiles == 0) return;
   const int per = (total + p.ctas - 1) / p.ctas;
   const int s0 = before + head * n_tiles, c0 = s0 / per, c1 = (s0 + n_tiles - 1) / per;
   if (c0 == c1) return;  // one run had all of it and has written the output
-  const int g = head / p.blocks, blk = head % p.blocks;
-  const int rows = min(kRows, p.group - blk * kRows), h0 = g * p.group + blk * kRows, D = p.c.D;
-  // slot of run c: the segment it starts in, unless the segment starts inside the run (or with it)
-  auto slot = [&](int c) { return 2 * int64_t(c) + (c == c0 ? 1 : 0); };
-  for (int i = threadIdx.x; i < rows * D; i += kConsumers) {
-    const int r = i / D, d = i - r * D;
-    float mx = -INFINITY;
-    for (int c = c0; c <= c1; c++) mx = fmaxf(mx, p.part_ml[(slot(c) * kRows + r) * 2]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, o = 0.f;
-    for (int c = c0; c <= c1; c++) {
-      const int64_t at = slot(c) * kRows + r;
-      const float f = ex2_approx(p.part_ml[at * 2] - base);
-      sum = fmaf(p.part_ml[at * 2 + 1], f, sum);
-      o = fmaf(p.part_o[at * DP + d], f, o);
+  // a part's slot: the one of the segment its run starts in, unless the work item starts inside the run (or with it)
+  auto slot = [&](int c) { return (2 * int64_t(c) + (c == c0 ? 1 : 0)) * kRows + r; };
+  float mx = -INFINITY;
+  for (int c = c0 + tid; c <= c1; c += kConsumers) mx = fmaxf(mx, p.part_ml[slot(c) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) top[warp] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f, o[kCh];
+#pragma unroll
+  for (int i = 0; i < kCh; i++) o[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += kWarps) {
+    const int64_t at = slot(c);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+    float v[kCh];
+    if (kCh == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * DP + 4 * lane);
+      v[0] = x.x, v[1] = x.y, v[kCh - 2] = x.z, v[kCh - 1] = x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * DP + 2 * lane);
+      v[0] = x.x, v[1] = x.y;
     }
-    const float res = sum > 0.f || sum != sum ? o / sum : 0.f;
-    p.a.out[(int64_t(b) * p.a.H + h0 + r) * D + d] = mxk_bf16(pack_bf16(res, 0.f) & 0xffffu);
-    if (d == 0 && p.a.lse) p.a.lse[int64_t(b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    const float f = ex2_approx(ml.x - base);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int i = 0; i < kCh; i++) o[i] = fmaf(v[i], f, o[i]);
   }
+#pragma unroll
+  for (int i = 0; i < kCh; i++) part[warp][lane * kCh + i] = o[i];
+  if (lane == 0) part_l[warp] = sum;
+  __syncthreads();
+  sum = part_l[0] + part_l[1] + part_l[2] + part_l[3];
+  const float f = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  if (tid < p.c.D)
+    p.a.out[(int64_t(b) * p.a.H + h) * p.c.D + tid] = mxk_bf16(pack_bf16((part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]) * f, 0.f) & 0xffffu);
+  if (tid == 0 && p.a.lse) p.a.lse[int64_t(b) * p.a.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
 template <bool E4M3, int DP>
@@ -627,7 +648,7 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
   launch_pdl(decode_kernel<E4M3, DP>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
   if (int rc = after_launch(name)) return rc;
-  launch_pdl(join_kernel<DP, DecodeCfg<E4M3, DP>::kTile>, dim3(unsigned(p.c.n_seqs * p.heads)), dim3(kConsumers), 0, s, p);
+  launch_pdl(join_kernel<DP, DecodeCfg<E4M3, DP>::kTile>, dim3(unsigned(p.c.n_seqs * p.heads), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
   return after_launch(name);
 }
 
