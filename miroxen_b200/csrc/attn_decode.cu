@@ -4,12 +4,12 @@
 //   s_j = scale * q . k_j,   m = max_j s_j,   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
 //
 // Every cached key and value in view is read once: 2 * Hkv * D elements per token against 4 * H * D flops, so memory
-// bounds it as long as the heads that share a key head are computed together.  They are the rows of the matrix
-// instructions here (mma.sync m16n8k16, up to 16 query heads of one key head; unused rows are zero): the tensor pipe is
-// far from busy at this ratio, and the operands come from shared memory tiles that change with every use, which is
-// what the warp-level instruction takes without a detour.
+// bounds it as long as the heads that share a key head are computed together.  They are the columns of the matrix
+// instructions here (mma.sync m16n8k16, 8 or 16 query heads of one key head; unused columns are zero): S^T = K Q^T, O^T =
+// V^T P^T.  The tensor pipe is far from busy at this ratio, and the operands come from shared memory tiles that change with
+// every use, which is what the warp-level instruction takes without a detour.
 //
-// Split: a tile is 64 or 128 tokens of one (sequence, key head, block of 16 query heads).  All tiles of the call in order
+// Split: a tile is 64 or 128 tokens of one (sequence, key head, block of query heads).  All tiles of the call in order
 // (sequence, head, token) are cut into equal runs, one per resident CTA, whatever the lengths are - a CTA's run may
 // end inside a sequence's tokens and cover several short sequences.  Each CTA finds the run's start itself by summing the
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
@@ -26,6 +26,8 @@
 // the tensor instruction needs the type of V.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "bulk_copy.cuh"
 #include "common.cuh"
 #include "kv_cache.cuh"
@@ -33,27 +35,22 @@
 namespace mxk {
 namespace {
 
-constexpr int kRows = 16;       // query heads per work item
 constexpr int kWarps = 4;       // that compute; one more copies
 constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32;
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
-#ifndef MXK_TOKW
-#define MXK_TOKW(E, DP) 16
-#define MXK_STAGES(E, DP) ((E) || (DP) == 64 ? 4 : 3)
-#endif
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DecodeLaunch {
   MxkDecodeArgs a;
   MxkKvCache c;
   int group;       // query heads per key head
-  int blocks;      // blocks of 16 of those
+  int blocks;      // blocks of 8 or 16 of those
   int heads;       // Hkv * blocks: work items per sequence
   int ctas;        // runs
   float scale2;    // scale * log2(e)
   unsigned page_recip;  // floor((2^32 - 1) / page_size)
-  float* part_o;   // [2 ctas][16][DP]
-  float* part_ml;  // [2 ctas][16][2]
+  float* part_o;   // [2 ctas][rows][DP], rows: query heads per block
+  float* part_ml;  // [2 ctas][rows][2]
   int* err;
 };
 
@@ -195,28 +192,31 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
 }
 
 // A stage holds a tile of K and one of V, a row per token, rows 16 bytes longer than their DP elements: the eight rows that
-// an ldmatrix phase reads then start four banks apart.  Tokens per tile and stages: about 32 KB a stage where a token's row
-// is long, twice the tokens where it is short, so that what a tile costs beside its bytes (a barrier, the vote, the
-// exchange of probabilities) is spread over as many.
+// an ldmatrix phase reads then start four banks apart.  A tile has 64 tokens, 16 for each computing warp: tiles of 128 tokens
+// cost the e4m3 kernels a CTA per SM and were slower or equal.  Stages: as many as leave two (bf16, D > 64) to four CTAs per
+// SM, whose number counts for more than the depth of a ring: 8 sequences of 32832 e4m3 tokens in view take 99.7 us with two
+// stages, 102.5 with three and 102.5 with four; 64 sequences of bf16, D = 128, 421 us with three stages, 455 with two,
+// 804 with four (one CTA per SM).
 template <bool E4M3, int DP>
 struct DecodeCfg {
-  static constexpr int kTokW = MXK_TOKW(E4M3, DP);  // tokens per warp
+  static constexpr int kTokW = 16;  // tokens per warp
   static constexpr int kTile = kTokW * kWarps;
   static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2), kPitch = kRowBytes + 16;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kTileBytes = kTile * kPitch;
-  static constexpr int kStages = MXK_STAGES(E4M3, DP);
+  static constexpr int kStages = DP == 64 ? 4 : E4M3 ? 2 : 3;
   static constexpr int kSmem = kStages * 2 * kTileBytes;
 };
 
-template <bool E4M3, int DP>
+// NH: blocks of 8 query heads.
+template <bool E4M3, int DP, int NH>
 __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant__ DecodeLaunch p) {
   using Cfg = DecodeCfg<E4M3, DP>;
   using elem = typename KvElem<E4M3>::type;
-  constexpr int kSt = Cfg::kStages, kTile = Cfg::kTile, kTokW = Cfg::kTokW, kPitch = Cfg::kPitch;
-  constexpr int kKSteps = DP / 16, kNW = DP / kWarps / 8, kNT = kTokW / 8;  // k-steps of the scores; 8-channel tiles, 8-token tiles per warp
+  constexpr int kSt = Cfg::kStages, kTile = Cfg::kTile, kTokW = Cfg::kTokW, kPitch = Cfg::kPitch, kRows = 8 * NH;
+  constexpr int kKSteps = DP / 16, kMT = DP / kWarps / 16, kTT = kTokW / 16;  // 16-channel steps, 16-channel tiles, 16-token tiles of a warp
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ __align__(16) unsigned short prob[2][kRows][kTile + 8];
+  __shared__ __align__(16) unsigned short prob[2][NH][kTile][8];  // [head block][token][head]
   __shared__ float wmax[kWarps][kRows], wsum[kWarps][kRows];
   __shared__ unsigned there[kSt][kTile / 32];  // which tokens of a tile exist
   __shared__ unsigned long long full[kSt], empty[kSt];
@@ -326,12 +326,12 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   }
 
   // ---- the computing warps ----
-  // this warp's state: rows r0 = lane / 4 and r0 + 8; channel tiles of the warp's quarter of the output
-  float o[kNW][4];
-  float base[2], l[2];  // maximum in use (in units of log2), this thread's part of the sum
-  unsigned qf[kKSteps][4];
-  float qs[2] = {1.f, 1.f}, ks2 = 0.f;
-  const int r0 = lane >> 2, c2 = (lane & 3) * 2;
+  // this warp's state.  Column c of a product is query head 8 nh + c; a lane holds columns 2 c2 and 2 c2 + 1 of rows r0 and
+  // r0 + 8 (tokens of the scores, channels of the output), as a right operand column r0.
+  float o[kMT][NH][4];
+  float base[NH][2], l[NH][2], scale[NH][2];  // maximum in use (in units of log2), this thread's part of the sum, of the columns
+  unsigned qf[NH][kKSteps][2];
+  const int r0 = lane >> 2, c2 = lane & 3;
   bool fresh = true;
   int first_tile = 0, st = 0, g = 0, rows = 0, h0 = 0;
   unsigned ph = 0;
@@ -342,49 +342,45 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       g = cur.head / p.blocks;
       const int blk = cur.head - g * p.blocks;
       rows = min(kRows, p.group - blk * kRows), h0 = g * p.group + blk * kRows;
-      ks2 = p.scale2 * (E4M3 && p.c.k_scale ? p.c.k_scale[g] : 1.f);
-#pragma unroll
-      for (int n = 0; n < kNW; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      base[0] = base[1] = -INFINITY, l[0] = l[1] = 0.f;
+      const float ks2 = p.scale2 * (E4M3 && p.c.k_scale ? p.c.k_scale[g] : 1.f);
       const mxk_bf16* q = p.a.q + int64_t(cur.b) * p.a.q_stride + int64_t(h0) * D;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const int r = r0 + 8 * half;
+      for (int nh = 0; nh < NH; nh++) {
+#pragma unroll
+        for (int m = 0; m < kMT; m++) o[m][nh][0] = o[m][nh][1] = o[m][nh][2] = o[m][nh][3] = 0.f;
+        base[nh][0] = base[nh][1] = -INFINITY, l[nh][0] = l[nh][1] = 0.f;
+        const int r = 8 * nh + r0;
         const bool on = r < rows;
-        if (!E4M3) {
+        // channels of step s: 16 s + 2 c2 + {0, 1} and + 8; of an e4m3 cache 16 s + 4 c2 + {0, 1} and {2, 3}, the order its
+        // keys are read in
+        float big = 0.f;
 #pragma unroll
-          for (int s = 0; s < kKSteps; s++)
+        for (int s = 0; s < kKSteps; s++)
 #pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-              const int d = 16 * s + 8 * hi + c2;
-              qf[s][half + 2 * hi] = on && d < D ? *reinterpret_cast<const unsigned*>(q + int64_t(r) * D + d) : 0u;
-            }
-        } else {
+          for (int hi = 0; hi < 2; hi++) {
+            const int d = 16 * s + (E4M3 ? 4 * c2 + 2 * hi : 2 * c2 + 8 * hi);
+            const unsigned x = on && d < D ? *reinterpret_cast<const unsigned*>(q + int64_t(r) * D + d) : 0u;
+            qf[nh][s][hi] = x;
+            if (E4M3) big = fmaxf(big, fmaxf(fabsf(bf16_lo(x)), fabsf(bf16_hi(x))));
+          }
+        float down = ks2;
+        if (E4M3) {
           // e4m3 keys are taken as f16, which holds them exactly; so are the queries, scaled by a power of two (per head)
-          // that brings their largest into [2^13, 2^14): what f16 then loses lies 2^-38 below it.  The order of channels in
-          // a 16-channel step is the one the keys are read in: lane c: channels 4 c + {0, 1 | 2, 3}.
-          unsigned raw[kKSteps][2];
-          float big = 0.f;
-#pragma unroll
-          for (int s = 0; s < kKSteps; s++)
-#pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-              const int d = 16 * s + 2 * c2 + 2 * hi;
-              raw[s][hi] = on && d < D ? *reinterpret_cast<const unsigned*>(q + int64_t(r) * D + d) : 0u;
-              big = fmaxf(big, fmaxf(fabsf(bf16_lo(raw[s][hi])), fabsf(bf16_hi(raw[s][hi]))));
-            }
+          // that brings their largest into [2^13, 2^14): what f16 then loses lies 2^-38 below it.
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
           // exponent of `big` by its bits; zero, subnormal and infinite rows keep a factor that changes nothing that matters
           int e = int((__float_as_uint(big) >> 23) & 255) - 127;
           e = e < -110 ? -110 : e > 127 ? 127 : e;
           const float up = __uint_as_float(unsigned(127 + 13 - e) << 23);
-          qs[half] = __uint_as_float(unsigned(127 - 13 + e) << 23);
+          down *= __uint_as_float(unsigned(127 - 13 + e) << 23);
 #pragma unroll
           for (int s = 0; s < kKSteps; s++)
 #pragma unroll
-            for (int hi = 0; hi < 2; hi++) qf[s][half + 2 * hi] = pack_f16(bf16_lo(raw[s][hi]) * up, bf16_hi(raw[s][hi]) * up);
+            for (int hi = 0; hi < 2; hi++) qf[nh][s][hi] = pack_f16(bf16_lo(qf[nh][s][hi]) * up, bf16_hi(qf[nh][s][hi]) * up);
         }
+        // the factor of head r0 goes to the lanes whose columns it is
+        scale[nh][0] = __shfl_sync(0xffffffffu, down, 8 * c2), scale[nh][1] = __shfl_sync(0xffffffffu, down, 8 * c2 + 4);
       }
     }
     // A wait that runs out does not leave the loop: the four warps go on meeting, without waiting for anything else.
@@ -392,117 +388,144 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     const unsigned k_u = ring_u + unsigned(st) * 2 * Cfg::kTileBytes, v_u = k_u + Cfg::kTileBytes;
 
     // ---- scores of this warp's tokens ----
-    float s[kNT][4];
+    float s[kTT][NH][4];
 #pragma unroll
-    for (int n = 0; n < kNT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int t = 0; t < kTT; t++)
+#pragma unroll
+      for (int nh = 0; nh < NH; nh++) s[t][nh][0] = s[t][nh][1] = s[t][nh][2] = s[t][nh][3] = 0.f;
     if (!E4M3) {
-      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
+      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 15)) * kPitch + (lane >> 4) * 16);
 #pragma unroll
       for (int ks = 0; ks < kKSteps; ks++)
 #pragma unroll
-        for (int n = 0; n < kNT; n += 2) {
-          unsigned b[4];
-          ldsm4(a + unsigned(n * 8 * kPitch + ks * 32), b);
-          mma16816<false>(s[n], qf[ks], b[0], b[1]);
-          mma16816<false>(s[n + 1], qf[ks], b[2], b[3]);
+        for (int t = 0; t < kTT; t++) {
+          unsigned k[4];
+          ldsm4(a + unsigned(t * 16 * kPitch + ks * 32), k);
+#pragma unroll
+          for (int nh = 0; nh < NH; nh++) mma16816<false>(s[t][nh], k, qf[nh][ks][0], qf[nh][ks][1]);
         }
     } else {
-      // four 16-byte chunks of 8 tokens: a register holds four channels of one token, two pairs of one 16-channel step
-      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 7)) * kPitch + (lane >> 3) * 16);
+      // two 16-byte chunks of 16 tokens: a register holds four channels of one token, two pairs of one 16-channel step
+      const unsigned a = k_u + unsigned((warp * kTokW + (lane & 15)) * kPitch + (lane >> 4) * 16);
 #pragma unroll
-      for (int grp = 0; grp < DP / 64; grp++)
+      for (int ks = 0; ks < kKSteps; ks += 2)
 #pragma unroll
-        for (int n = 0; n < kNT; n++) {
+        for (int t = 0; t < kTT; t++) {
           unsigned w[4];
-          ldsm4(a + unsigned(n * 8 * kPitch + grp * 64), w);
+          ldsm4(a + unsigned(t * 16 * kPitch + ks * 16), w);
 #pragma unroll
-          for (int ks = 0; ks < 4; ks++) mma16816<true>(s[n], qf[4 * grp + ks], e4m3x2_to_f16x2(w[ks] & 0xffffu), e4m3x2_to_f16x2(w[ks] >> 16));
+          for (int x = 0; x < 2; x++) {
+            const unsigned k[4] = {e4m3x2_to_f16x2(w[2 * x] & 0xffffu), e4m3x2_to_f16x2(w[2 * x + 1] & 0xffffu), e4m3x2_to_f16x2(w[2 * x] >> 16),
+                                   e4m3x2_to_f16x2(w[2 * x + 1] >> 16)};
+#pragma unroll
+            for (int nh = 0; nh < NH; nh++) mma16816<true>(s[t][nh], k, qf[nh][ks + x][0], qf[nh][ks + x][1]);
+          }
         }
     }
     // the warp's bits of the tile's tokens
     const unsigned word = there[st][warp * kTokW / 32] >> (warp * kTokW % 32);
-    const bool all_there = kTokW == 32 ? word == 0xffffffffu : (word & 0xffffu) == 0xffffu;
-    const float f0 = E4M3 ? ks2 * qs[0] : ks2, f1 = E4M3 ? ks2 * qs[1] : ks2;
+    const bool all_there = (word & 0xffffu) == 0xffffu;
+    float mx[NH][2];
+    bool grows = false;
 #pragma unroll
-    for (int n = 0; n < kNT; n++) s[n][0] *= f0, s[n][1] *= f0, s[n][2] *= f1, s[n][3] *= f1;
-    if (!all_there) {
+    for (int nh = 0; nh < NH; nh++) {
 #pragma unroll
-      for (int n = 0; n < kNT; n++)
+      for (int t = 0; t < kTT; t++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (!(word >> (8 * n + c2 + (e & 1)) & 1u)) s[n][e] = -INFINITY;
+        for (int e = 0; e < 4; e++) {
+          s[t][nh][e] *= scale[nh][e & 1];
+          if (!all_there && !(word >> (16 * t + 8 * (e >> 1) + r0) & 1u)) s[t][nh][e] = -INFINITY;
+        }
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        mx[nh][c] = fmaxf(s[0][nh][c], s[0][nh][2 + c]);
+#pragma unroll
+        for (int t = 1; t < kTT; t++) mx[nh][c] = fmaxf(mx[nh][c], fmaxf(s[t][nh][c], s[t][nh][2 + c]));
+        grows |= mx[nh][c] > base[nh][c] + kSlack;
+      }
     }
-    float mx[2] = {fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])};
-#pragma unroll
-    for (int n = 1; n < kNT; n++) mx[0] = fmaxf(mx[0], fmaxf(s[n][0], s[n][1])), mx[1] = fmaxf(mx[1], fmaxf(s[n][2], s[n][3]));
-    unsigned short(*pr)[kTile + 8] = prob[i & 1];
-    float add[2];
+    float add[NH][2];
     auto probabilities = [&]() {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const float b = base[h] == -INFINITY ? 0.f : base[h];  // nothing seen yet: exp2(-inf - 0) = 0 everywhere
-        add[h] = 0.f;
+      for (int nh = 0; nh < NH; nh++) {
+        const float b0 = base[nh][0] == -INFINITY ? 0.f : base[nh][0];  // nothing seen yet: exp2(-inf - 0) = 0 everywhere
+        const float b1 = base[nh][1] == -INFINITY ? 0.f : base[nh][1];
+        add[nh][0] = add[nh][1] = 0.f;
 #pragma unroll
-        for (int n = 0; n < kNT; n++) {
-          const float p0 = ex2_approx(s[n][2 * h] - b), p1 = ex2_approx(s[n][2 * h + 1] - b);
-          add[h] += p0 + p1;
-          *reinterpret_cast<unsigned*>(&pr[r0 + 8 * h][warp * kTokW + 8 * n + c2]) = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
-        }
+        for (int t = 0; t < kTT; t++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const float p0 = ex2_approx(s[t][nh][2 * half] - b0), p1 = ex2_approx(s[t][nh][2 * half + 1] - b1);
+            add[nh][0] += p0, add[nh][1] += p1;
+            *reinterpret_cast<unsigned*>(&prob[i & 1][nh][warp * kTokW + 16 * t + 8 * half + r0][2 * c2]) = E4M3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+          }
       }
     };
     probabilities();
-    if (vote(mx[0] > base[0] + kSlack || mx[1] > base[1] + kSlack)) {  // always in a segment's first tile
+    if (vote(grows)) {  // always in a segment's first tile
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        if ((lane & 3) == 0) wmax[warp][r0 + 8 * h] = mx[h];
-      }
+      for (int nh = 0; nh < NH; nh++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[nh][c] = fmaxf(mx[nh][c], __shfl_xor_sync(0xffffffffu, mx[nh][c], x));
+          if (r0 == 0) wmax[warp][8 * nh + 2 * c2 + c] = mx[nh][c];
+        }
       meet();
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float mn = base[h];
+      for (int nh = 0; nh < NH; nh++)
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) mn = fmaxf(mn, wmax[w][r0 + 8 * h]);
-        if (mn != base[h]) {
-          const float f = ex2_approx(base[h] - mn);  // 0 for the first maximum
-          l[h] *= f;
+        for (int c = 0; c < 2; c++) {
+          float mn = base[nh][c];
 #pragma unroll
-          for (int n = 0; n < kNW; n++) o[n][2 * h] *= f, o[n][2 * h + 1] *= f;
-          base[h] = mn;
+          for (int w = 0; w < kWarps; w++) mn = fmaxf(mn, wmax[w][8 * nh + 2 * c2 + c]);
+          if (mn != base[nh][c]) {
+            const float f = ex2_approx(base[nh][c] - mn);  // 0 for the first maximum
+            l[nh][c] *= f;
+#pragma unroll
+            for (int m = 0; m < kMT; m++) o[m][nh][c] *= f, o[m][nh][2 + c] *= f;
+            base[nh][c] = mn;
+          }
         }
-      }
       probabilities();
       meet();
     }
-    l[0] += add[0], l[1] += add[1];
+#pragma unroll
+    for (int nh = 0; nh < NH; nh++) l[nh][0] += add[nh][0], l[nh][1] += add[nh][1];
     // ---- this warp's channels of the product with V ----
-    const unsigned pa_u = smem_u32(&pr[(lane & 7) + (((lane >> 3) & 1) << 3)][(lane >> 4) << 3]);
-    const unsigned va_u = v_u + unsigned(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch) +
-                          unsigned((E4M3 ? (kNW / 2 == 2 ? warp * 2 + (lane >> 4) : warp) : warp * kNW + (lane >> 4)) * 16);
+    const unsigned p_u = smem_u32(&prob[i & 1][0][lane][0]);
 #pragma unroll
-    for (int ks = 0; ks < kTile / 16; ks++) {
-      unsigned pa[4];
-      ldsm4(pa_u + unsigned(ks * 32), pa);
+    for (int k2 = 0; k2 < kTile / 32; k2++) {  // 32 tokens, two steps
+      unsigned pb[NH][4];
+#pragma unroll
+      for (int nh = 0; nh < NH; nh++) ldsm4_t(p_u + unsigned((nh * kTile + k2 * 32) * 16), pb[nh]);
       if (!E4M3) {
+        const unsigned a = v_u + unsigned((k2 * 32 + (lane & 7) + ((lane >> 4) << 3)) * kPitch + (warp * kMT * 2 + ((lane >> 3) & 1)) * 16);
 #pragma unroll
-        for (int n = 0; n < kNW; n += 2) {
-          unsigned b[4];
-          ldsm4_t(va_u + unsigned(ks * 16 * kPitch + n * 16), b);
-          mma16816<false>(o[n], pa, b[0], b[1]);
-          mma16816<false>(o[n + 1], pa, b[2], b[3]);
-        }
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+          for (int m = 0; m < kMT; m++) {
+            unsigned v[4];
+            ldsm4_t(a + unsigned(ks * 16 * kPitch + m * 32), v);
+#pragma unroll
+            for (int nh = 0; nh < NH; nh++) mma16816<false>(o[m][nh], v, pb[nh][2 * ks], pb[nh][2 * ks + 1]);
+          }
       } else {
-        // a 16-bit transposed load of 8-bit pairs: register: (token 2c: channels 2n, 2n + 1), (token 2c + 1: the same);
-        // the pairs of one channel are then its bytes 0, 2 and 1, 3, so two channel tiles hold the even and the odd ones
-        constexpr int kPairs = kNW / 2;  // 16-byte chunks of the warp (16 channels each)
-        unsigned b[4];
-        ldsm4_t(va_u + unsigned(ks * 16 * kPitch), b);
+        // A 16-bit transposed load of 8-bit pairs: register: (token 2c: channels 2n, 2n + 1), (token 2c + 1: the same); the
+        // pairs of one channel are then its bytes 0, 2 and 1, 3: rows 0-7 of the product take the even channels of the 16,
+        // rows 8-15 the odd ones.
 #pragma unroll
-        for (int n = 0; n < kPairs; n++) {
-          const unsigned lo = b[2 * n], hi = b[2 * n + 1];  // tokens 0-7 and 8-15 of the step
-          mma16816<true>(o[2 * n], pa, e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4420)));
-          mma16816<true>(o[2 * n + 1], pa, e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4431)), e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4431)));
+        for (int m = 0; m < kMT; m++) {
+          unsigned v[4];  // tokens 0-7, 8-15, 16-23, 24-31
+          ldsm4_t(v_u + unsigned((k2 * 32 + lane) * kPitch + (warp * kMT + m) * 16), v);
+#pragma unroll
+          for (int ks = 0; ks < 2; ks++) {
+            const unsigned lo = v[2 * ks], hi = v[2 * ks + 1];
+            const unsigned a[4] = {e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4431)),
+                                   e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4431))};
+#pragma unroll
+            for (int nh = 0; nh < NH; nh++) mma16816<true>(o[m][nh], a, pb[nh][2 * ks], pb[nh][2 * ks + 1]);
+          }
         }
       }
     }
@@ -514,44 +537,49 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     if (last || i + 1 == n_my) {  // the (sequence, head) or the run ends: store
       const bool whole = last && first_tile == 0;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if ((lane & 3) == 0) wsum[warp][r0 + 8 * h] = l[h];
-      }
+      for (int nh = 0; nh < NH; nh++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[nh][c] += __shfl_xor_sync(0xffffffffu, l[nh][c], x);
+          if (r0 == 0) wsum[warp][8 * nh + 2 * c2 + c] = l[nh][c];
+        }
       meet();
       const float vs = E4M3 && p.c.v_scale ? p.c.v_scale[g] : 1.f;
+      const int64_t slot = 2 * int64_t(blockIdx.x) + (first_tile == 0 ? 1 : 0);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int r = r0 + 8 * h;
-        if (r >= rows) continue;
-        float sum = 0.f;
+      for (int nh = 0; nh < NH; nh++)
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) sum += wsum[w][r];
-        const int64_t slot = 2 * int64_t(blockIdx.x) + (first_tile == 0 ? 1 : 0);
-        const float f = whole ? (sum > 0.f || sum != sum ? vs / sum : 0.f) : vs;
+        for (int c = 0; c < 2; c++) {
+          const int r = 8 * nh + 2 * c2 + c;
+          if (r >= rows) continue;
+          float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < kNW; n++) {
-          // channels of o[n][2h], o[n][2h + 1]
-          const int d0 = E4M3 ? (warp * (kNW / 2) + n / 2) * 16 + 2 * c2 + (n & 1) : (warp * kNW + n) * 8 + c2, d1 = E4M3 ? d0 + 2 : d0 + 1;
-          if (whole) {
-            mxk_bf16* dst = p.a.out + (int64_t(cur.b) * p.a.H + h0 + r) * D;
-            const unsigned w = pack_bf16(o[n][2 * h] * f, o[n][2 * h + 1] * f);
-            if (d0 < D) dst[d0] = mxk_bf16(w & 0xffffu);
-            if (d1 < D) dst[d1] = mxk_bf16(w >> 16);
-          } else {
-            float* dst = p.part_o + (slot * kRows + r) * DP;
-            dst[d0] = o[n][2 * h] * f, dst[d1] = o[n][2 * h + 1] * f;
+          for (int w = 0; w < kWarps; w++) sum += wsum[w][r];
+          const float f = whole ? (sum > 0.f || sum != sum ? vs / sum : 0.f) : vs;
+#pragma unroll
+          for (int m = 0; m < kMT; m++) {
+            // channels of o[m][nh][c] and o[m][nh][2 + c]
+            const int d0 = (warp * kMT + m) * 16 + (E4M3 ? 2 * r0 : r0), d1 = E4M3 ? d0 + 1 : d0 + 8;
+            const float v0 = o[m][nh][c] * f, v1 = o[m][nh][2 + c] * f;
+            if (whole) {
+              mxk_bf16* dst = p.a.out + (int64_t(cur.b) * p.a.H + h0 + r) * D;
+              const unsigned w = pack_bf16(v0, v1);
+              if (d0 < D) dst[d0] = mxk_bf16(w & 0xffffu);
+              if (d1 < D) dst[d1] = mxk_bf16(w >> 16);
+            } else {
+              float* dst = p.part_o + (slot * kRows + r) * DP;
+              dst[d0] = v0, dst[d1] = v1;
+            }
+          }
+          if (warp == 0 && r0 == 0) {
+            if (!whole) {
+              p.part_ml[(slot * kRows + r) * 2] = base[nh][c], p.part_ml[(slot * kRows + r) * 2 + 1] = sum;
+            } else if (p.a.lse) {
+              p.a.lse[int64_t(cur.b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (base[nh][c] + log2f(sum)) * kLn2;
+            }
           }
         }
-        if (warp == 0 && (lane & 3) == 0) {
-          if (!whole) {
-            p.part_ml[(slot * kRows + r) * 2] = base[h], p.part_ml[(slot * kRows + r) * 2 + 1] = sum;
-          } else if (p.a.lse) {
-            p.a.lse[int64_t(cur.b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (base[h] + log2f(sum)) * kLn2;
-          }
-        }
-      }
       fresh = true;
     }
     cursor_next<kTile>(p, cur);
@@ -562,8 +590,9 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
 // Adds up, for each (sequence, head) that several runs share, the parts in the order of the runs: one CTA per work item and
 // row, warp w taking parts w, w + 4, ... (all channels of a part per access, several parts in flight), the warps' sums in
 // order at the end.
-template <int DP, int TILE>
+template <int DP, int TILE, int NH>
 __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant__ DecodeLaunch p) {
+  constexpr int kRows = 8 * NH;
   constexpr int kCh = DP / 32;  // channels of a lane
   __shared__ int sums[2][kWarps];
   __shared__ float top[kWarps], part_l[kWarps], part[kWarps][DP];
@@ -631,25 +660,36 @@ __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant_
   if (tid == 0 && p.a.lse) p.a.lse[int64_t(b) * p.a.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-template <bool E4M3, int DP>
+template <bool E4M3, int DP, int NH>
 int decode_ctas() {
-  auto k = decode_kernel<E4M3, DP>;
+  auto k = decode_kernel<E4M3, DP, NH>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<E4M3, DP>::kSmem);
   return sm_count() * resident_ctas(k, kThreadsD, DecodeCfg<E4M3, DP>::kSmem);
 }
 
-template <bool E4M3, int DP>
+template <bool E4M3, int DP, int NH>
 int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
-  p.ctas = decode_ctas<E4M3, DP>();
+  constexpr int kRows = 8 * NH, kTile = DecodeCfg<E4M3, DP>::kTile;
+  p.ctas = decode_ctas<E4M3, DP, NH>();
   // no more runs than there can be tiles
-  const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, DecodeCfg<E4M3, DP>::kTile);
+  const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, kTile);
   if (p.ctas > most) p.ctas = int(most < 1 ? 1 : most);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
-  launch_pdl(decode_kernel<E4M3, DP>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
+  launch_pdl(decode_kernel<E4M3, DP, NH>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
   if (int rc = after_launch(name)) return rc;
-  launch_pdl(join_kernel<DP, DecodeCfg<E4M3, DP>::kTile>, dim3(unsigned(p.c.n_seqs * p.heads), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
+  launch_pdl(join_kernel<DP, kTile, NH>, dim3(unsigned(p.c.n_seqs * p.heads), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
   return after_launch(name);
+}
+
+// The kernel for a cache and head count: f(e4m3, padded head dimension, blocks of 8 heads), as types.
+template <int N> using Int = std::integral_constant<int, N>;
+template <class F>
+auto pick_decode(const MxkKvCache* c, int group, F f) {
+  const bool e = c->type == MXK_KV_E4M3, small = c->D <= 64;
+  auto with_heads = [&](auto type, auto dp) { return group <= 8 ? f(type, dp, Int<1>()) : f(type, dp, Int<2>()); };
+  if (e) return small ? with_heads(Int<1>(), Int<64>()) : with_heads(Int<1>(), Int<128>());
+  return small ? with_heads(Int<0>(), Int<64>()) : with_heads(Int<0>(), Int<128>());
 }
 
 int check_heads(const char* name, const MxkKvCache* c, int H) {
@@ -668,11 +708,11 @@ int64_t mxk_attn_decode_workspace_bytes(const MxkKvCache* cache, int H) {
   const char* name = "attn_decode_workspace_bytes";
   if (int rc = check_cache(name, cache)) return rc;
   if (int rc = check_heads(name, cache, H)) return rc;
-  const bool e = cache->type == MXK_KV_E4M3;
-  const int dp = cache->D <= 64 ? 64 : 128;
-  const int ctas = dp == 64 ? (e ? decode_ctas<true, 64>() : decode_ctas<false, 64>()) : (e ? decode_ctas<true, 128>() : decode_ctas<false, 128>());
-  cudaGetLastError();
-  return int64_t(2) * ctas * kRows * (dp + 2) * int64_t(sizeof(float));
+  const int64_t bytes = pick_decode(cache, H / cache->Hkv, [](auto e, auto dp, auto nh) {
+    return int64_t(2) * decode_ctas<e.value != 0, dp.value, nh.value>() * (8 * nh.value) * (dp.value + 2) * int64_t(sizeof(float));
+  });
+  cudaGetLastError();  // without a GPU the size is that of the usual one
+  return bytes;
 }
 
 int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mxk_stream_t stream) {
@@ -693,7 +733,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   if (a.sinks < 0) return fail(MXK_ERR_INVALID_ARG, "%s: sinks=%lld", name, (long long)a.sinks);
   if (!(a.scale > 0.f) || a.scale > 3.0e38f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and finite", name);
   p.group = a.H / cache->Hkv;
-  p.blocks = int(ceil_div(p.group, kRows));
+  p.blocks = int(ceil_div(p.group, 16));
   p.heads = cache->Hkv * p.blocks;
   const int64_t tiles = int64_t(cache->n_seqs) * p.heads * (ceil_div(int64_t(cache->max_pages) * cache->page_size, 64) + 1);
   if (tiles >= (int64_t(1) << 30)) return fail(MXK_ERR_TOO_LARGE, "%s: n_seqs * heads * tokens too large (%lld tiles)", name, (long long)tiles);
@@ -701,8 +741,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   p.page_recip = 0xffffffffu / unsigned(cache->page_size);
   p.err = device_error_word();
   const cudaStream_t s = as_stream(stream);
-  if (cache->D <= 64) return cache->type == MXK_KV_E4M3 ? launch_decode<true, 64>(name, p, s) : launch_decode<false, 64>(name, p, s);
-  return cache->type == MXK_KV_E4M3 ? launch_decode<true, 128>(name, p, s) : launch_decode<false, 128>(name, p, s);
+  return pick_decode(cache, p.group, [&](auto e, auto dp, auto nh) { return launch_decode<e.value != 0, dp.value, nh.value>(name, p, s); });
 }
 
 }  // extern "C"
