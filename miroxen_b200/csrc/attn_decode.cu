@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant_
 template <bool E4M3, int DP, int NH>
 int decode_ctas() {
   auto k = decode_kernel<E4M3, DP, NH>;
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<E4M3, DP>::kSmem);
+  allow_smem(k, DecodeCfg<E4M3, DP>::kSmem);  // a failure surfaces at the launch
   return sm_count() * resident_ctas(k, kThreadsD, DecodeCfg<E4M3, DP>::kSmem);
 }
 

@@ -723,7 +723,7 @@ int launch_window(const char* name, WindowLaunch& W, cudaStream_t s) {
   if (int rc = make_map(name, &mv, a.k_rows > 0 ? a.v : a.q, a.k_rows > 0 ? a.k_rows : 1, a.k_rows > 0 ? a.Hkv : 1, a.D, a.v_stride)) return rc;
   auto k = window_kernel<DP>;
   const size_t smem = sizeof(WindowSmem<DP>);
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  const cudaError_t e = allow_smem(k, smem);
   if (e != cudaSuccess) return fail(MXK_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(e));
   const int64_t ctas = int64_t(W.max_tiles) * a.H;
   if (ctas >= (int64_t(1) << 31)) return fail(MXK_ERR_TOO_LARGE, "%s: %lld tiles", name, (long long)ctas);

@@ -32,6 +32,14 @@ inline int resident_ctas(K kernel, int threads, size_t smem = 0) {
   return resident_ctas_lookup(reinterpret_cast<const void*>(kernel), threads, smem);
 }
 
+// Lets `kernel` have `smem` bytes of dynamic shared memory on the current device; the runtime is asked once per kernel and
+// device (half a microsecond otherwise, on every launch).
+cudaError_t allow_smem_lookup(const void* kernel, size_t smem);
+template <class K>
+inline cudaError_t allow_smem(K kernel, size_t smem) {
+  return allow_smem_lookup(reinterpret_cast<const void*>(kernel), smem);
+}
+
 // Programmatic dependent launch: a kernel launched through launch_pdl() may be scheduled while the
 // previous kernel of the stream is still draining; its threads park at pdl_wait() until that kernel
 // has completed and its writes are visible, so only work that touches no global memory (barrier

@@ -108,6 +108,31 @@ int resident_ctas_lookup(const void* kernel, int threads, size_t smem) {
   return n;
 }
 
+namespace {
+// Kernel and device, in one word each so that a slot is claimed by one exchange; slots are never given back.
+std::atomic<uint64_t> g_smem_set[256];
+}  // namespace
+
+cudaError_t allow_smem_lookup(const void* kernel, size_t smem) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t key = (uint64_t(reinterpret_cast<uintptr_t>(kernel)) << 8) | uint64_t(dev + 1);  // addresses have 56 bits at most
+  unsigned h = unsigned((key * 0x9e3779b97f4a7c15ull) >> 56);
+  for (int probe = 0; probe < 256; probe++, h = (h + 1) & 255u) {
+    const uint64_t k = g_smem_set[h].load(std::memory_order_acquire);
+    if (k == key) return cudaSuccess;
+    if (k == 0) break;
+  }
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  for (int probe = 0; probe < 256; probe++, h = (h + 1) & 255u) {
+    uint64_t expect = 0;
+    if (g_smem_set[h].compare_exchange_strong(expect, key, std::memory_order_acq_rel) || expect == key) break;
+  }
+  return cudaSuccess;
+}
+
 bool pdl_enabled() { return g_tune[TUNE_PDL].load(std::memory_order_relaxed) != 2; }
 
 int tune(int key, int dflt) {

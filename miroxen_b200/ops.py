@@ -45,8 +45,15 @@ def _p(t) -> Optional[int]:
     return t.data_ptr()
 
 
+# The current stream's handle without a Stream object around it (0.3 instead of 3.2 us per call, which is most of what a
+# short kernel takes); the public way where a build of torch does not have it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream) -> Optional[int]:
     if stream is None:
+        if _raw_stream is not None and torch.cuda.is_initialized():
+            return _raw_stream(torch.cuda.current_device()) or None
         return torch.cuda.current_stream().cuda_stream or None
     if isinstance(stream, int):
         return stream or None
@@ -355,9 +362,16 @@ class KvCache:
         if any(t is not None and t.device != k.device for t in (v, page_table, k_scale, v_scale)):
             raise MxkError("KvCache: all tensors must be on one device")
         self.k, self.v, self.page_table, self.k_scale, self.v_scale = k, v, page_table, k_scale, v_scale
+        self._index = k.get_device()  # -1: not on a GPU
         self._args = KvCacheArgs(_p(k), _p(v), _p(page_table), _p(k_scale), _p(v_scale), k.shape[0], k.stride(0), k.stride(1),
                                  k.stride(2), page_table.stride(0), page_table.shape[0], page_table.shape[1], k.shape[1],
                                  k.shape[2], k.shape[3], KV_BF16 if k.dtype == torch.bfloat16 else KV_E4M3)
+
+
+def _here(what, index):
+    """The library works on the current device; a tensor of another one is refused before its address gets there."""
+    if index >= 0 and index != torch.cuda.current_device():
+        raise MxkError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
 
 
 def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, table_rows, rot, mode, cache: KvCache, positions,
@@ -366,6 +380,7 @@ def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, ta
     c = cache._args
     if D != c.D:
         raise MxkError(f"qkv_norm_rope_append: D={D} and a cache of D={c.D}")
+    _here("qkv_norm_rope_append", cache._index)
     kv = c.Hkv * D
     a = AppendArgs(_p(q), _p(k), _p(v), T, H * D if q_stride is None else q_stride, kv if k_stride is None else k_stride,
                    kv if v_stride is None else v_stride, _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), table_rows, _p(positions),
@@ -376,6 +391,7 @@ def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, ta
 def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
     """Scratch memory for attn_decode_paged with this cache and head count: keep one for each stream or graph that may
     run at the same time as another."""
+    _here("attn_decode_workspace", cache._index)
     n = lib().mxk_attn_decode_workspace_bytes(cache._args, H)
     if n < 0:
         check(n)
@@ -385,6 +401,7 @@ def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
 def attn_decode_paged(q, cache: KvCache, seq_lens, H, scale, out, left=-1, sinks=0, q_stride=None, lse=None, *, workspace, stream=None):
     """Attention of one new token of every sequence over its tokens in the cache."""
     c = cache._args
+    _here("attn_decode_paged", cache._index)
     a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), left, sinks, H, scale)
     check(lib().mxk_attn_decode_paged(a, c, _stream(stream)))
 
@@ -395,6 +412,8 @@ def attn_window(q, k, v, q_rows, k_rows, H, Hkv, D, scale, out, left=-1, right=-
     window of `left` / `right` keys (-1: no bound; right = 0: causal) and `sinks` first keys that stay visible."""
     if n_seqs is None:
         n_seqs = 1 if cu_q is None else cu_q.numel() - 1
+    if not isinstance(q, int):
+        _here("attn_window", q.get_device())
     a = AttnArgs(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k), q_rows, k_rows, H * D if q_stride is None else q_stride,
                  Hkv * D if k_stride is None else k_stride, Hkv * D if v_stride is None else v_stride,
                  H * D if out_stride is None else out_stride, left, right, sinks, n_seqs, H, Hkv, D, scale)
