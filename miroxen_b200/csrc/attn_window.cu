@@ -13,7 +13,8 @@
 //                   probabilities go back as bf16 (the type of V, which the product needs);
 //   warps 8, 10:    issue tcgen05.mma: S = Q K^T from shared memory (8), O += P V with P from tensor memory (10);
 //   warp 9:         TMA: Q once, then the tiles of K and V through a ring of shared-memory stages (128-byte swizzle);
-//   warp 11:        only completes the group of four whose registers the softmax warps take over (setmaxnreg).
+//   warp 11:        finds the tiles: the CTA's own, then those of CTAs that have not started (cluster launch control).
+// A tile's loads, first products and its search run while the tile before it is finished.
 // Tensor memory: one score tile (128 columns), which the halves use in turn, the probabilities P of each half (64) and the
 // output O of each half (128), 512 in all.  A score tile is free as soon as its half has it in registers, so the tensor pipe
 // makes the next one, and the products with V, while the softmax runs: S0 | S1 | S0' P0 V | S1' P1 V | ...  Nothing goes
@@ -127,11 +128,16 @@ __device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------
 
 constexpr int kM = 128, kN = 128;              // rows of a half, keys of a block
-constexpr int kScoreWarp = 8, kTmaWarp = 9, kValueWarp = 10, kThreadsW = 384;
+constexpr int kScoreWarp = 8, kTmaWarp = 9, kValueWarp = 10, kScheduleWarp = 11, kThreadsW = 384;
+constexpr int kReaders = kThreadsW / 32 - 1;    // warps that are told the tiles
 constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channel tile
 // Registers a thread: 384 x 168 at launch; a softmax thread holds 128 scores, the others need fewer.
 constexpr int kRegsSoft = 208, kRegsOther = 88;
 static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
+#ifndef MXK_ASK
+#define MXK_ASK 6
+#endif
+constexpr int kAskAhead = MXK_ASK;             // loads of a tile that are still to come when the next tile is asked for
 constexpr unsigned kTmemS = 0, kTmemP = 128, kTmemO = 256, kTmemCols = 512;  // S, 2 x 64 of P, 2 x 128 of O
 constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
 
@@ -139,17 +145,7 @@ template <int DP>
 struct WindowCfg {
   static constexpr int kSubs = DP / 64;               // 64-channel tiles of a row
   static constexpr int kTileBytes = kSubs * kSub;     // Q half, K block, V block
-  static constexpr int kStages = DP == 128 ? 5 : 8;
-};
-
-template <int DP>
-struct __align__(1024) WindowSmem {
-  unsigned char q[2][WindowCfg<DP>::kTileBytes];
-  unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
-  unsigned long long q_full[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2];
-  unsigned tmem_base;
-  int poison[2];  // a value that is not finite lies in a block at the edge of the half's view
-  int scan[kThreadsW / 32], found[6];
+  static constexpr int kStages = DP == 128 ? 4 : 8;
 };
 
 __device__ __forceinline__ void tma_load_3d(unsigned dst, const CUtensorMap* map, int c0, int c1, int c2, unsigned bar) {
@@ -301,55 +297,117 @@ struct WindowLaunch {
   int max_tiles;  // the grid has max_tiles * H CTAs
 };
 
-// What a CTA works on: rows [r0, r0 + rows) of a sequence that starts at row q0 / key k0 and has nq rows, nk keys.
+// What a tile is: rows [r0, r0 + rows) and head `head` of a sequence that starts at row q0 / key k0 and has nq rows, nk keys.
+// rows = 0: there is no further one.
 struct WindowTile {
-  int q0, nq, k0, nk, r0, rows;
+  int q0, nq, k0, nk, r0, rows, head;
 };
 
-// Tile `want` counted over the sequences, with the whole CTA; rows = 0: there is none.
-__device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int want, int* scan, int* found) {
+// Tile number `cta` of the launch, by one warp; rows = 0 if there is no such tile.  The tiles at the end of a causal sequence,
+// which have the most keys, come first, all heads of a tile one behind the other: the other way round, head by head, the CTAs
+// at work crowd on the same few lines of the keys (packed prompts XX against YY us).
+__device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta) {
   const MxkAttnArgs& a = W.L.a;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, tile_rows = kM * W.halves;
-  WindowTile t{0, int(a.q_rows), 0, int(a.k_rows), 0, 0};
+  const int lane = threadIdx.x & 31, tile_rows = kM * W.halves;
+  const int place = cta / a.H, want = W.max_tiles - 1 - place;
+  WindowTile t{0, int(a.q_rows), 0, int(a.k_rows), 0, 0, cta - place * a.H};
   if (!a.cu_q) {
     t.r0 = want * tile_rows;
     t.rows = min(tile_rows, t.nq - t.r0);
     return t;
   }
-  // thread t counts a contiguous share of the sequences; the ends of its first one (its only one, mostly) stay in registers
-  const int n = a.n_seqs, share = (n + kThreadsW - 1) / kThreadsW, b0 = min(n, tid * share), b1 = min(n, b0 + share);
-  int mine = 0, q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-  auto ends = [&](int b) {
-    const int x0 = a.cu_q[b], x1 = a.cu_q[b + 1], y0 = a.cu_k[b], y1 = a.cu_k[b + 1];
-    // held inside the arrays and in order whatever they hold
-    q0 = max(0, min(x0, int(a.q_rows))), q1 = max(q0, min(x1, int(a.q_rows)));
-    k0 = max(0, min(y0, int(a.k_rows))), k1 = max(k0, min(y1, int(a.k_rows)));
-    if ((q0 != x0 || q1 != x1 || k0 != y0 || k1 != y1) && W.L.err) atomicExch(W.L.err, kErrBadIndex);
-    return (q1 - q0 + tile_rows - 1) / tile_rows;
-  };
-  for (int b = b1 - 1; b >= b0; b--) mine += ends(b);
-  int incl = mine;
+  constexpr int kAhead = 4;  // groups of 32 sequences whose ends are asked for at once
+  int at = 0;                // tiles of the sequences in front
+  for (int base = 0; base < a.n_seqs; base += 32 * kAhead) {
+    int x[kAhead][4];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
+    for (int u = 0; u < kAhead; u++) {
+      const int b = base + 32 * u + lane;
+      x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0;
+      if (b < a.n_seqs) x[u][0] = a.cu_q[b], x[u][1] = a.cu_q[b + 1], x[u][2] = a.cu_k[b], x[u][3] = a.cu_k[b + 1];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      if (base + 32 * u >= a.n_seqs) break;
+      // held inside the arrays and in order whatever they hold
+      const int q0 = max(0, min(x[u][0], int(a.q_rows))), q1 = max(q0, min(x[u][1], int(a.q_rows)));
+      const int k0 = max(0, min(x[u][2], int(a.k_rows))), k1 = max(k0, min(x[u][3], int(a.k_rows)));
+      if ((q0 != x[u][0] || q1 != x[u][1] || k0 != x[u][2] || k1 != x[u][3]) && W.L.err) atomicExch(W.L.err, kErrBadIndex);
+      const int mine = (q1 - q0 + tile_rows - 1) / tile_rows;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const int first = at + incl - mine;
+      const unsigned hit = __ballot_sync(0xffffffffu, want >= first && want < first + mine);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        t.q0 = __shfl_sync(0xffffffffu, q0, src), t.nq = __shfl_sync(0xffffffffu, q1 - q0, src);
+        t.k0 = __shfl_sync(0xffffffffu, k0, src), t.nk = __shfl_sync(0xffffffffu, k1 - k0, src);
+        t.r0 = (want - __shfl_sync(0xffffffffu, first, src)) * tile_rows;
+        t.rows = min(tile_rows, t.nq - t.r0);
+        return t;
+      }
+      at += __shfl_sync(0xffffffffu, incl, 31);
+    }
   }
-  if (lane == 31) scan[warp] = incl;
-  if (tid == 0) found[5] = 0;
-  __syncthreads();
-  int at = incl - mine;
-  for (int w = 0; w < warp; w++) at += scan[w];
-  if (want >= at && want < at + mine) {
-    int b = b0;
-    if (share > 1)
-      for (int k = ends(b); want >= at + k; k = ends(b)) at += k, b++;
-    found[0] = q0, found[1] = q1 - q0, found[2] = k0, found[3] = k1 - k0, found[4] = (want - at) * tile_rows, found[5] = 1;
-  }
-  __syncthreads();
-  if (!found[5]) return t;
-  t.q0 = found[0], t.nq = found[1], t.k0 = found[2], t.nk = found[3], t.r0 = found[4];
-  t.rows = min(tile_rows, t.nq - t.r0);
   return t;
+}
+
+template <int DP>
+struct __align__(1024) WindowSmem {
+  unsigned char q[2][WindowCfg<DP>::kTileBytes];
+  unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
+  unsigned char stage[2][kSub];  // the halves' output on its way to memory, 64 channels at a time
+  unsigned long long q_full[2], q_empty[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2], o_empty[2],
+      tile_full[2], tile_empty[2], wanted, asked, marks_seen[2];
+  uint4 answer[1];
+  WindowTile tile[2];
+  unsigned tmem_base;
+  int poison[2][2];  // [half][number of its outputs & 1]: a value that is not finite lies in a block at the edge of the half's view
+};
+
+// The blocks of 128 keys that a tile's rows see.
+struct TileView {
+  int halves, shift;     // a row's position is its number + shift
+  Seen first[2], end[2];  // of the first and the last row of each half: the nearest end, the farthest window start
+  int wb0, n_sink, n_blocks;
+  __device__ __forceinline__ TileView(const AttnLaunch& L, const WindowTile& t) {
+    halves = t.rows > kM ? 2 : 1;
+    shift = t.nk - t.nq;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      first[h] = seen_by(L, t.r0 + h * kM + shift, t.nk);
+      end[h] = seen_by(L, t.r0 + min((h + 1) * kM, t.rows) - 1 + shift, t.nk);
+    }
+    const Seen s = first[0], e = halves == 2 ? end[1] : end[0];
+    wb0 = s.lo / kN;  // the tile's blocks: n_sink from the front, the others from wb0 on
+    n_sink = min((e.first + kN - 1) / kN, wb0);
+    n_blocks = n_sink + (e.hi > s.lo ? (e.hi + kN - 1) / kN - wb0 : 0);
+  }
+  __device__ __forceinline__ int block(int j) const { return j < n_sink ? j : wb0 + j - n_sink; }
+  // whether some row of half h sees keys of the block; the last such block, -1 if there is none
+  __device__ __forceinline__ int last(int h) const { return h >= halves ? -1 : end[h].hi > first[h].lo ? (end[h].hi - 1) / kN : (end[h].first + kN - 1) / kN - 1; }
+  __device__ __forceinline__ bool has(int h, int b) const { return b <= last(h) && (b * kN < end[h].first || b >= first[h].lo / kN); }
+};
+
+// Asks the hardware for a CTA of this launch that has not started; its number, or -1 when there is none left.  The answer lands
+// in shared memory (16 bytes) and completes `bar`.
+__device__ __forceinline__ void ask_for_tile(unsigned answer, unsigned bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int tile_answer(unsigned answer) {
+  int x = -1;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%1];\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n\t}"
+      : "+r"(x)
+      : "r"(answer)
+      : "memory");
+  return x;
 }
 
 template <int DP>
@@ -364,103 +422,133 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   const AttnLaunch& L = W.L;
   const MxkAttnArgs& a = L.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  // Head by head, so that the CTAs at work read the keys of few heads and at about the same time; the tiles at the end of a
-  // causal sequence, which have the most keys, first.
-  const int head = int(blockIdx.x) / W.max_tiles, want = W.max_tiles - 1 - int(blockIdx.x) % W.max_tiles, kv_head = head / L.group;
-
-  if (tid == 0) {
-    for (int i = 0; i < 2; i++) {
-      mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.pv_done[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), 4);
-      sm.poison[i] = 0;
-    }
-    mbar_init(smem_u32(&sm.s_free), 4);
-    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  pdl_launch_dependents();
-  pdl_wait();
-  const WindowTile t = find_tile(W, want, sm.scan, sm.found);
-  if (t.rows <= 0) return;  // the whole CTA
   if (smem_u32(smem_raw) & 1023u) {  // never seen; nothing is computed on tiles that the swizzle would not fit
     if (tid == 0 && L.err) atomicExch(L.err, kErrBulkTimeout);
     return;
   }
-  const int halves = t.rows > kM ? 2 : 1;
 
-  // blocks of keys that some row of the tile sees: n_sink from the front, the others from block wb0 on
-  const int shift = t.nk - t.nq;  // a row's position is its number + shift
-  const Seen s_first = seen_by(L, t.r0 + shift, t.nk), s_last = seen_by(L, t.r0 + t.rows - 1 + shift, t.nk);
-  const int wb0 = s_first.lo / kN, wb1 = s_last.hi > s_first.lo ? (s_last.hi + kN - 1) / kN : wb0;
-  const int n_sink = min((s_last.first + kN - 1) / kN, wb0);
-  const int n_blocks = n_sink + wb1 - wb0;
-  auto block_at = [&](int j) { return j < n_sink ? j : wb0 + j - n_sink; };
-  // which blocks some row of half h sees: those in front of `sinks`, and [from, last]
-  struct HalfView {
-    int sinks, from, last;
-    __device__ __forceinline__ bool has(int block) const { return block <= last && (block < sinks || block >= from); }
-  } view[2];
-  int first_block[2];  // its place in the order of the tile's blocks
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const Seen f = seen_by(L, t.r0 + h * kM + shift, t.nk), e = seen_by(L, t.r0 + min((h + 1) * kM, t.rows) - 1 + shift, t.nk);
-    view[h].from = f.lo / kN;
-    view[h].sinks = (e.first + kN - 1) / kN;
-    view[h].last = e.hi > f.lo ? (e.hi - 1) / kN : view[h].sinks - 1;
-    first_block[h] = view[h].sinks > 0 ? 0 : view[h].from - wb0 + n_sink;
-    if (h >= halves) view[h].last = -1;
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.q_empty[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1);
+      mbar_init(smem_u32(&sm.pv_done[i]), 1), mbar_init(smem_u32(&sm.p_full[i]), 4), mbar_init(smem_u32(&sm.o_empty[i]), 4);
+      mbar_init(smem_u32(&sm.tile_full[i]), 1), mbar_init(smem_u32(&sm.tile_empty[i]), kReaders);
+      mbar_init(smem_u32(&sm.marks_seen[i]), 4);
+      sm.poison[i][0] = sm.poison[i][1] = 0;
+    }
+    mbar_init(smem_u32(&sm.s_free), 4), mbar_init(smem_u32(&sm.asked), 1), mbar_init(smem_u32(&sm.wanted), 1);
+    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-
   if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_launch_dependents();
   fence_before();
   __syncthreads();
   fence_after();
   const unsigned tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
+  pdl_wait();  // nothing above touches global memory
 
+  // Every wait is bounded; a role whose wait runs out leaves its loop, the others' waits then run out too.
   bool ok = true;
-  int issued = 0;  // TMA lane: stage fills issued so far
+  auto wait = [&](unsigned long long* bar, int phase) {
+    const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(bar), unsigned(phase) & 1u));
+    fence_after();
+    return r;
+  };
+  // The n-th tile of this CTA, from the ring of two that the scheduling warp fills; false: there is none (or the wait ran out).
+  auto next_tile = [&](int n, WindowTile& t) {
+    ok = wait(&sm.tile_full[n & 1], n >> 1);
+    if (!ok) return false;
+    t = sm.tile[n & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(smem_u32(&sm.tile_empty[n & 1]));
+    return t.rows > 0;
+  };
+  int issued = 0, q_issued[2] = {0, 0};  // TMA: stage and Q fills so far
+
   if (warp >= kScoreWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == kTmaWarp && lane == 0 && n_blocks > 0) {
-      for (int h = 0; h < halves; h++) {
-        const unsigned bar = smem_u32(&sm.q_full[h]);
-        mbar_expect_tx(bar, Cfg::kTileBytes);
-        for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.q[h]) + c * kSub, &map_q, c * 64, head, t.q0 + t.r0 + h * kM, bar);
-      }
-      // fill 2 j: K of block j; fill 2 j + 1: its V
-      for (issued = 0; issued < 2 * n_blocks; issued++) {
-        const int st = issued % kSt;
-        if (issued >= kSt && !mbar_wait_spin(smem_u32(&sm.empty[st]), unsigned(issued / kSt - 1) & 1u)) {
-          ok = false;
-          break;
+    const unsigned leader = elect_lane();
+    WindowTile t;
+    if (warp == kScheduleWarp) {
+      // ---- which tiles: this CTA's own, then those of CTAs that have not started yet.  One is asked for when the loads of
+      // the tile at hand come to their end, no earlier: what a CTA has asked for no other can take at the end of the launch.
+      int cta = int(blockIdx.x), n = 0;
+      for (int asks = 0; ok; asks++) {
+        t = find_tile(W, cta);
+        if (t.rows > 0) {
+          if (n >= 2) ok = wait(&sm.tile_empty[n & 1], (n >> 1) - 1);
+          if (ok && leader) {
+            sm.tile[n & 1] = t;
+            mbar_arrive1(smem_u32(&sm.tile_full[n & 1]));
+          }
+          __syncwarp();
+          if (ok) ok = wait(&sm.wanted, n);
+          n++;
         }
-        const unsigned bar = smem_u32(&sm.full[st]);
-        mbar_expect_tx(bar, Cfg::kTileBytes);
-        const int key = t.k0 + block_at(issued >> 1) * kN;
-        const CUtensorMap* map = (issued & 1) ? &map_v : &map_k;
-        for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.kv[st]) + c * kSub, map, c * 64, kv_head, key, bar);
+        if (!ok) break;
+        if (leader) ask_for_tile(smem_u32(sm.answer), smem_u32(&sm.asked));
+        ok = wait(&sm.asked, asks);
+        cta = ok ? tile_answer(smem_u32(sm.answer)) : -1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before it is written over
+        __syncwarp();
+        if (cta < 0) break;
       }
-    } else if ((warp == kScoreWarp || warp == kValueWarp) && n_blocks > 0) {
-      const unsigned leader = elect_lane();
-      auto wait = [&](unsigned long long* bar, int phase) {
-        const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(bar), unsigned(phase) & 1u));
-        fence_after();
-        return r;
-      };
-      // A half passes over blocks that none of its rows sees.
-      if (warp == kScoreWarp) {
-        int made = 0;  // score tiles so far
-        for (int j = 0; j < n_blocks && ok; j++) {
-          const int block = block_at(j), fill = 2 * j;
+      if (ok && n >= 2) ok = wait(&sm.tile_empty[n & 1], (n >> 1) - 1);
+      if (ok && leader) {
+        sm.tile[n & 1].rows = 0;
+        mbar_arrive1(smem_u32(&sm.tile_full[n & 1]));
+      }
+    } else if (warp == kTmaWarp) {
+      for (int n = 0; next_tile(n, t); n++) {
+        const TileView v(L, t);
+        const int kv_head = t.head / L.group;
+        auto load_q = [&](int h) {
+          if (v.last(h) < 0) return;
+          if (q_issued[h] > 0 && ok) ok = wait(&sm.q_empty[h], q_issued[h] - 1);
+          if (!ok) return;
+          const unsigned bar = smem_u32(&sm.q_full[h]);
+          if (leader) {
+            mbar_expect_tx(bar, Cfg::kTileBytes);
+            for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.q[h]) + c * kSub, &map_q, c * 64, t.head, t.q0 + t.r0 + h * kM, bar);
+          }
+          q_issued[h]++;
+        };
+        // in the order in which they are needed: Q of the first half, K, Q of the second half, V, ...
+        const int n_fills = 2 * v.n_blocks, want_at = max(0, n_fills - kAskAhead);
+        if (n_fills == 0 && leader) mbar_arrive1(smem_u32(&sm.wanted));
+        for (int i = 0; i < n_fills && ok; i++) {  // 2 j: K of block j; 2 j + 1: its V
+          if (i == want_at && leader) mbar_arrive1(smem_u32(&sm.wanted));
+          if (i < 2) load_q(i);
+          const int st = issued % kSt;
+          if (ok && issued >= kSt) ok = wait(&sm.empty[st], issued / kSt - 1);
+          if (!ok) break;
+          const unsigned bar = smem_u32(&sm.full[st]);
+          const int key = t.k0 + v.block(i >> 1) * kN;
+          if (leader) {
+            mbar_expect_tx(bar, Cfg::kTileBytes);
+            const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
+            for (int c = 0; c < Cfg::kSubs; c++) tma_load_3d(smem_u32(sm.kv[st]) + c * kSub, map, c * 64, kv_head, key, bar);
+          }
+          issued++;
+        }
+        if (!ok) break;
+      }
+    } else if (warp == kScoreWarp) {
+      int fill0 = 0, made = 0, q_used[2] = {0, 0};  // fills in front of this tile, score tiles, Q tiles so far
+      for (int n = 0; next_tile(n, t); n++) {
+        const TileView v(L, t);
+        bool fresh[2] = {true, true};
+        for (int j = 0; j < v.n_blocks && ok; j++) {
+          const int block = v.block(j), fill = fill0 + 2 * j;
           ok = wait(&sm.full[fill % kSt], fill / kSt);
           const unsigned ka = smem_u32(sm.kv[fill % kSt]);
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            if (h >= halves || !ok || !view[h].has(block)) continue;
-            if (j == first_block[h]) ok = wait(&sm.q_full[h], 0);
+            if (!ok || !v.has(h, block)) continue;
+            if (fresh[h]) ok = wait(&sm.q_full[h], q_used[h]), fresh[h] = false;
             if (ok && made > 0) ok = wait(&sm.s_free, made - 1);  // the tile before this one is in its half's registers
             if (!ok) continue;
             const unsigned qa = smem_u32(sm.q[h]);
@@ -472,58 +560,83 @@ __global__ void __launch_bounds__(kThreadsW, 1)
                        kInstr<kM, kN, false>, (c | k) != 0 ? 1u : 0u, leader);
             commit_to(smem_u32(&sm.s_full[h]), leader);
             made++;
+            if (block == v.last(h)) commit_to(smem_u32(&sm.q_empty[h]), leader), q_used[h]++;
           }
           if (ok) commit_to(smem_u32(&sm.empty[fill % kSt]), leader);
         }
-      } else {
-        int done[2] = {0, 0};  // blocks a half has had
-        for (int j = 0; j < n_blocks && ok; j++) {
-          const int block = block_at(j), fill = 2 * j + 1;
+        if (!ok) break;
+        fill0 += 2 * v.n_blocks;
+      }
+    } else if (warp == kValueWarp) {
+      int fill0 = 0, done[2] = {0, 0}, used[2] = {0, 0};  // fills in front of this tile; blocks and outputs a half has had
+      for (int n = 0; next_tile(n, t); n++) {
+        const TileView v(L, t);
+        bool fresh[2] = {true, true};
+        for (int j = 0; j < v.n_blocks && ok; j++) {
+          const int block = v.block(j), fill = fill0 + 2 * j + 1;
           ok = wait(&sm.full[fill % kSt], fill / kSt);
           const unsigned va = smem_u32(sm.kv[fill % kSt]);
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            if (h >= halves || !ok || !view[h].has(block)) continue;
-            ok = wait(&sm.p_full[h], done[h]);
+            if (!ok || !v.has(h, block)) continue;
+            if (fresh[h] && used[h] > 0) ok = wait(&sm.o_empty[h], used[h] - 1);  // the output of the tile before is in registers
+            if (ok) ok = wait(&sm.p_full[h], done[h]);
             if (!ok) continue;
 #pragma unroll
             for (int k = 0; k < kN / 16; k++)  // 16 keys: 8 columns of P, 2048 bytes of V
               mma_ts(tmem + kTmemO + unsigned(h) * 128, tmem + kTmemP + unsigned(h) * 64 + unsigned(k) * 8, desc_sw128(va, kSub) + uint64_t(k * 128),
-                     kInstr<kM, DP, true>, k > 0 || done[h] > 0 ? 1u : 0u, leader);
+                     kInstr<kM, DP, true>, k > 0 || !fresh[h] ? 1u : 0u, leader);
             commit_to(smem_u32(&sm.pv_done[h]), leader);
-            done[h]++;
+            done[h]++, fresh[h] = false;
           }
           if (ok) commit_to(smem_u32(&sm.empty[fill % kSt]), leader);
         }
+        if (!ok) break;
+        fill0 += 2 * v.n_blocks;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (!fresh[h]) used[h]++;
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
-    if ((warp >> 2) < halves) {
-      // ---- softmax of half h: thread (warp & 3) * 32 + lane owns that row ----
-      const int h = warp >> 2, row_h = (warp & 3) * 32 + lane, rh0 = t.r0 + h * kM;
-      const int rows_h = min(kM, t.rows - h * kM);
-      const unsigned lanes = unsigned((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + lanes + kTmemS, tp = tmem + lanes + kTmemP + unsigned(h) * 64, to = tmem + lanes + kTmemO + unsigned(h) * 128;
-      const Seen mine = seen_by(L, min(rh0 + row_h, t.nq - 1) + shift, t.nk);
-      // the first row of the half has the nearest end, the last row the farthest window start
-      const Seen h_first = seen_by(L, rh0 + shift, t.nk), h_last = seen_by(L, rh0 + rows_h - 1 + shift, t.nk);
-      const HalfView blocks = h == 0 ? view[0] : view[1];
+    // ---- softmax of half h: thread (warp & 3) * 32 + lane owns that row ----
+    const int h = warp >> 2, row_h = (warp & 3) * 32 + lane;
+    const unsigned lanes = unsigned((warp & 3) * 32) << 16;
+    const unsigned ts = tmem + lanes + kTmemS, tp = tmem + lanes + kTmemP + unsigned(h) * 64, to = tmem + lanes + kTmemO + unsigned(h) * 128;
+    unsigned char* stage = sm.stage[h] + (warp & 3) * (32 * 128);  // 32 rows of 64 channels on their way out
+    int fill0 = 0, all = 0, used = 0, marks = 0;  // fills in front of this tile; blocks, outputs and marked outputs that the half has had
+    for (int n = 0;; n++) {
+      // The tile stays this warp's until its output is done; what the loop over the blocks does not need is read again behind it
+      // (a row of scores leaves few registers).
+      ok = wait(&sm.tile_full[n & 1], n >> 1);
+      if (!ok) break;
+      const WindowTile& tile = sm.tile[n & 1];
+      if (tile.rows <= 0) break;
+      int blocks, wb0, n_sink, last, from, sinks, full_from, full_sinks, full_to;
+      {
+        const WindowTile t = tile;
+        const TileView v(L, t);
+        const Seen f = h == 0 ? v.first[0] : v.first[1], e = h == 0 ? v.end[0] : v.end[1];
+        blocks = v.n_blocks, wb0 = v.wb0, n_sink = v.n_sink;
+        last = h == 0 ? v.last(0) : v.last(1);                         // blocks that some row of the half sees: as TileView::has
+        from = f.lo / kN, sinks = (e.first + kN - 1) / kN;
+        full_from = (e.lo + kN - 1) / kN, full_sinks = f.first / kN, full_to = f.hi / kN;  // blocks that all its rows see all of
+      }
       float m = -INFINITY, l = 0.f;  // maximum in use (of the raw scores), sum
-      int done = 0;                  // blocks that some row of the half sees, so far
-      for (int j = 0; j < n_blocks; j++) {
-        const int block = block_at(j);
-        if (!blocks.has(block)) continue;
-        const int key0 = block * kN;
-        const bool edge = !(key0 + kN <= h_first.hi && (key0 >= h_last.lo || key0 + kN <= h_first.first));
+      int done = 0;                  // blocks of this tile that some row of the half sees, so far
+      for (int j = 0; j < blocks; j++) {
+        const int block = j < n_sink ? j : wb0 + j - n_sink;
+        if (!(block <= last && (block < sinks || block >= from))) continue;
+        const bool edge = !(block < full_to && (block >= full_from || block < full_sinks));
         // A wait that runs out: the warp goes on without waiting for anything else.  Its lanes agree on the outcome.
         if (edge) {
           // V of this block, before the scores are there: zero what lies behind the sequence, look for values that are not
           // finite in the rest (an exponent of all ones carries into the sign bit when one is added to it)
-          const int fv = 2 * j + 1;
+          const int fv = fill0 + 2 * j + 1;
           ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u));
           uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
-          const int there = t.nk - key0;
+          const int there = tile.nk - block * kN;
           unsigned odd = 0;
           if (ok) {
 #pragma unroll
@@ -535,14 +648,14 @@ __global__ void __launch_bounds__(kThreadsW, 1)
               if (((i * kM + row_h) >> 3) % kN < there) odd |= y;
             }
           }
-          if (odd & 0x80008000u) sm.poison[h] = 1;
+          if (odd & 0x80008000u) sm.poison[h][used & 1] = 1;
           if (ok && there < kN) {
             for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM)
               if ((i >> 3) % kN >= there) vt[i] = make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(done) & 1u));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(all) & 1u));
         fence_after();
         unsigned s[4][32];
 #pragma unroll
@@ -555,9 +668,10 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         if (edge) {
           // bit i of below(n): i < n
           auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+          const Seen mine = seen_by(L, min(tile.r0 + h * kM + row_h, tile.nq - 1) + tile.nk - tile.nq, tile.nk);
 #pragma unroll
           for (int c = 0; c < 4; c++) {
-            const int k0 = key0 + 32 * c;
+            const int k0 = block * kN + 32 * c;
             const unsigned see = below(mine.first - k0) | (below(mine.hi - k0) & ~below(mine.lo - k0));
 #pragma unroll
             for (int i = 0; i < 32; i++) s[c][i] = (see >> i) & 1u ? s[c][i] : 0xff800000u;
@@ -584,7 +698,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             m = mx, l *= f;
           }
           if (done > 0 && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u));
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u));
             fence_after();
 #pragma unroll 1
             for (int c = 0; c < DP / 16; c++) {
@@ -601,7 +715,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         // P is the product's until it has retired
         auto wait_p = [&]() {
           if (done > 0 && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u));
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u));
             fence_after();
           }
         };
@@ -624,42 +738,75 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         }
         if (ok) hand_over(&sm.p_full[h], lane);
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        done++;
+        done++, all++;
       }
+      fill0 += 2 * blocks;
       // ---- output ----
-      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(done - 1) & 1u);
+      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        fence_after();
-        const int64_t row = int64_t(t.q0) + rh0 + row_h;
-        const bool on = row_h < rows_h;
-        if (done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h])) {
-          float* qs = reinterpret_cast<float*>(sm.q[h]) + (warp & 3) * MXK_ATTN_MAX_HEAD_DIM;  // Q is not needed any more
-          for (int r = (warp & 3) * 32; r < min((warp & 3) * 32 + 32, rows_h); r++)
-            row_attention(L, int64_t(t.q0) + rh0 + r, head, t.k0, rh0 + r + shift, t.nk, qs);
-        } else {
-          const bool some = l > 0.f || l != l;
-          const float f = some ? 1.f / l : 0.f;
-          mxk_bf16* dst = a.out + row * a.out_stride + int64_t(head) * a.D;
+      if (!ok) break;
+      fence_after();
+      const WindowTile t = tile;
+      const int rh0 = t.r0 + h * kM + (warp & 3) * 32, rows_w = min(32, t.rows - (rh0 - t.r0));  // of this warp, none if negative
+      const int64_t row0 = int64_t(t.q0) + rh0;
+      const bool poisoned = done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h][used & 1]);
+      const bool some = l > 0.f || l != l;
+      const float f = some ? 1.f / l : 0.f;
 #pragma unroll 1
-          for (int c = 0; c < DP / 32; c++) {
-            unsigned o[32];
-            if (done > 0) {
-              tmem_ld32(to + 32 * c, o);
-              tmem_wait_ld(o);
-            }
-            if (!on) continue;
+      for (int c = 0; c < DP / 64; c++) {
+        unsigned o[2][32];
+        if (done == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              float v[8];
-#pragma unroll
-              for (int e = 0; e < 8; e++) v[e] = some ? __uint_as_float(o[8 * i + e]) * f : 0.f;
-              if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * i) = pack8(v);
-            }
+          for (int i = 0; i < 32; i++) o[0][i] = o[1][i] = 0u;
+        } else {
+          tmem_ld32(to + 64 * c, o[0]);
+          tmem_ld32(to + 64 * c + 32, o[1]);
+          tmem_wait_ld(o[0]);
+          tmem_touch(o[1]);
+          if (c == DP / 64 - 1) {  // the next tile's output may come
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive1(smem_u32(&sm.o_empty[h]));
           }
-          if (on && a.lse) a.lse[row * a.H + head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
         }
+        // A row per lane from tensor memory, 128 bytes of four rows per store to memory: through shared memory, the 16-byte
+        // chunks of a row exchanged by the row's number.
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = __uint_as_float(o[i >> 2][8 * (i & 3) + e]) * f;  // 0 * 0 in a row that sees nothing
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) = pack8(x);
+        }
+        __syncwarp();
+        if (!poisoned) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int r = 4 * i + (lane >> 3), ch = 64 * c + 8 * (lane & 7);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+            if (r < rows_w && ch < a.D) *reinterpret_cast<uint4*>(a.out + (row0 + r) * a.out_stride + int64_t(t.head) * a.D + ch) = x;
+          }
+        }
+        __syncwarp();
       }
+      if (!poisoned && a.lse && lane < rows_w)
+        a.lse[(row0 + lane) * a.H + t.head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
+      if (poisoned) {
+        for (int r = 0; r < rows_w; r++)
+          row_attention(L, row0 + r, t.head, t.k0, rh0 + r + t.nk - t.nq, t.nk, reinterpret_cast<float*>(stage));
+        // The mark is taken back once the half's four warps have seen it.  Nobody sets it again before: that takes another
+        // tile's product with V in between, which needs the probabilities of all four.
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(smem_u32(&sm.marks_seen[h]));
+        if ((warp & 3) == 0) {
+          ok = wait(&sm.marks_seen[h], marks);
+          if (lane == 0) sm.poison[h][used & 1] = 0;
+        }
+        marks++;
+      }
+      if (done > 0) used++;
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(smem_u32(&sm.tile_empty[n & 1]));
     }
   }
 
@@ -668,8 +815,9 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   // Every role's waits are bounded, so all threads arrive here.  After a failure the copies under way get a bounded chance
   // to land before the shared memory goes.
   if (__syncthreads_or(!ok) != 0) {
-    if (tid == kTmaWarp * 32) {
-      for (int h = 0; h < halves; h++) mbar_wait(smem_u32(&sm.q_full[h]), 0);
+    if (warp == kTmaWarp) {
+      for (int h = 0; h < 2; h++)
+        if (q_issued[h] > 0) mbar_wait(smem_u32(&sm.q_full[h]), unsigned(q_issued[h] - 1) & 1u);
       for (int i = issued > kSt ? issued - kSt : 0; i < issued; i++) mbar_wait(smem_u32(&sm.full[i % kSt]), unsigned(i / kSt) & 1u);
     }
     __syncthreads();
