@@ -24,9 +24,9 @@
 // The running maximum that the exponentials use moves only when it would grow by more than 2^8 (results are the same:
 // every sum is relative to it), so O is rescaled rarely, by the half's own warps, once its products so far have retired.
 // Blocks of 128 keys outside of every row's view are not visited; only blocks at the edge of some row's view pay for the
-// mask.  There, what lies out of view must not reach 0 * v: value rows behind the sequence are zeroed in shared memory, and
-// if any other value of the block is not finite the rows are taken again by a plain loop (row_attention) that never touches
-// what a row does not see.
+// mask.  There, what a row does not see still takes part in the product as 0 * v, which is not 0 where v is not finite: an
+// output that is not finite has its rows' edge blocks looked through, and if it can have come from there the row is taken
+// again by a plain loop (row_attention) that never touches what the row does not see.
 #include <cuda.h>
 
 #include <atomic>
@@ -63,7 +63,7 @@ __device__ __forceinline__ Seen seen_by(const AttnLaunch& L, int p, int nk) {
 
 // One row and head by one warp, 32 keys at a time: a lane takes a key's product with q, then the warp adds the keys'
 // values, each lane holding channels 2 lane, 2 lane + 1, + 64.  `qs`: the warp's 128 floats of shared memory.
-__device__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k0, int p, int nk, float* qs) {
+__device__ __forceinline__ void row_attention(const AttnLaunch& L, int64_t row, int h, int64_t k0, int p, int nk, float* qs) {
   const MxkAttnArgs& a = L.a;
   const int lane = threadIdx.x & 31, D = a.D, g = h / L.group;
   const Seen seen = seen_by(L, p, nk);
@@ -132,12 +132,9 @@ constexpr int kScoreWarp = 8, kTmaWarp = 9, kValueWarp = 10, kScheduleWarp = 11,
 constexpr int kReaders = kThreadsW / 32 - 1;    // warps that are told the tiles
 constexpr int kSub = 128 * 128;                // bytes of a 128-row x 64-channel tile
 // Registers a thread: 384 x 168 at launch; a softmax thread holds 128 scores, the others need fewer.
-constexpr int kRegsSoft = 208, kRegsOther = 88;
+constexpr int kRegsSoft = 216, kRegsOther = 72;
 static_assert(256 * kRegsSoft + 128 * kRegsOther <= kThreadsW * 168, "the groups' registers are those of the launch");
-#ifndef MXK_ASK
-#define MXK_ASK 6
-#endif
-constexpr int kAskAhead = MXK_ASK;             // loads of a tile that are still to come when the next tile is asked for
+constexpr int kAskAhead = 6;                   // loads of a tile that are still to come when the next tile is asked for
 constexpr unsigned kTmemS = 0, kTmemP = 128, kTmemO = 256, kTmemCols = 512;  // S, 2 x 64 of P, 2 x 128 of O
 constexpr float kSlack = 8.f;                  // log2 of how far a score may lie above the maximum in use
 
@@ -245,50 +242,38 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {  // NaN if
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of N values on the multiply-add pipe, for -126 <= x < 127: x = n + f, |f| <= 1/2, n by adding and taking away 1.5 * 2^23
-// (the integer then stands in the low bits), 2^f by a polynomial of degree 5 fitted to the least relative error on
-// [-1/2, 1/2] (7.5e-8, below the hardware's 2^x), n added to its exponent.
-template <int N>
-__device__ __forceinline__ void exp2_poly(float (&x)[N]) {
-  constexpr float c[6] = {1.3276472454890609e-3f, 9.675540961325169e-3f, 5.550713092088699e-2f, 0.24022120237350464f, 0.6931469440460205f, 1.0000001192092896f};
-  float r[N], f[N], p[N];
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = fmaxf(x[i], -126.f), r[i] = x[i] + 12582912.f;
-#pragma unroll
-  for (int i = 0; i < N; i++) f[i] = x[i] - (r[i] - 12582912.f), p[i] = fmaf(f[i], c[0], c[1]);
-#pragma unroll
-  for (int k = 2; k < 6; k++)
-#pragma unroll
-    for (int i = 0; i < N; i++) p[i] = fmaf(p[i], f[i], c[k]);
-#pragma unroll
-  for (int i = 0; i < N; i++) x[i] = __uint_as_float(__float_as_uint(p[i]) + (__float_as_uint(r[i]) << 23));
+// Pairs of fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
 }
-#ifndef MXK_POLY
-#define MXK_POLY 0
-#endif
-constexpr int kPoly = MXK_POLY;  // of 32 scores this many take their 2^x on the multiply-add pipe
+__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 // Probabilities of 32 scores: p = 2^(s * scale2 - base), their sum into l (four partial sums), rounded to bf16 in pairs.
-template <bool POLY>
-__device__ __forceinline__ void exp_chunk(const unsigned (&s)[32], float scale2, float base, float (&l)[4], unsigned (&p)[16]) {
-  constexpr int N = POLY ? kPoly : 0;
-  float x[32];
+// Pairs of fp32 operations where there are any: single ones take 367 instead of 363 us on 2 x 4352 rows x 24 heads and 129
+// instead of 121 us on the packed prompts.  (Some of the 2^x as polynomials beside the special-function unit, which is busy
+// two thirds of the time, made the kernel slower in proportion to their number, in every form tried: its warps and, in long
+// runs, its power have less to spare than that unit.)
+__device__ __forceinline__ void exp_chunk(const unsigned (&s)[32], uint64_t scale2, uint64_t neg_base, uint64_t (&l)[2], unsigned (&p)[16]) {
 #pragma unroll
-  for (int i = 0; i < 32; i++) x[i] = fmaf(__uint_as_float(s[i]), scale2, -base);
-  if constexpr (N > 0) {
-    float y[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) y[i] = x[i];
-    exp2_poly(y);
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = y[i];
+  for (int i = 0; i < 16; i++) {
+    float x, y;
+    split(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, neg_base), x, y);
+    x = ex2_approx(x), y = ex2_approx(y);
+    l[i & 1] = add2(l[i & 1], pair(x, y));
+    p[i] = pack_bf16(x, y);
   }
-#pragma unroll
-  for (int i = N; i < 32; i++) x[i] = ex2_approx(x[i]);
-#pragma unroll
-  for (int i = 0; i < 32; i++) l[i & 3] += x[i];
-#pragma unroll
-  for (int i = 0; i < 16; i++) p[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
 }
 
 struct WindowLaunch {
@@ -362,11 +347,10 @@ struct __align__(1024) WindowSmem {
   unsigned char kv[WindowCfg<DP>::kStages][WindowCfg<DP>::kTileBytes];
   unsigned char stage[2][kSub];  // the halves' output on its way to memory, 64 channels at a time
   unsigned long long q_full[2], q_empty[2], full[WindowCfg<DP>::kStages], empty[WindowCfg<DP>::kStages], s_full[2], s_free, p_full[2], pv_done[2], o_empty[2],
-      tile_full[2], tile_empty[2], wanted, asked, marks_seen[2];
+      tile_full[2], tile_empty[2], wanted, asked;
   uint4 answer[1];
   WindowTile tile[2];
   unsigned tmem_base;
-  int poison[2][2];  // [half][number of its outputs & 1]: a value that is not finite lies in a block at the edge of the half's view
 };
 
 // The blocks of 128 keys that a tile's rows see.
@@ -392,6 +376,29 @@ struct TileView {
   __device__ __forceinline__ int last(int h) const { return h >= halves ? -1 : end[h].hi > first[h].lo ? (end[h].hi - 1) / kN : (end[h].first + kN - 1) / kN - 1; }
   __device__ __forceinline__ bool has(int h, int b) const { return b <= last(h) && (b * kN < end[h].first || b >= first[h].lo / kN); }
 };
+
+// Whether a block of keys that some row of half h of the tile sees only a part of holds a value that is not finite, in any of
+// its 128 rows (those behind the sequence too: they have been loaded with it).  By one warp, and rarely.
+__device__ __forceinline__ bool hidden_value_odd(const AttnLaunch& L, const WindowTile& t, int h) {
+  const MxkAttnArgs& a = L.a;
+  const TileView v(L, t);
+  const Seen f = h == 0 ? v.first[0] : v.first[1], e = h == 0 ? v.end[0] : v.end[1];
+  const int lane = threadIdx.x & 31, chunks = a.D / 8;
+  const mxk_bf16* vb = a.v + int64_t(t.head / L.group) * a.D;
+  bool odd = false;
+  for (int j = 0; j < v.n_blocks; j++) {
+    const int block = v.block(j), key0 = block * kN;
+    if (!(h == 0 ? v.has(0, block) : v.has(1, block)) || (key0 + kN <= f.hi && (key0 >= e.lo || key0 + kN <= f.first))) continue;
+    const int rows = int(min(int64_t(kN), a.k_rows - t.k0 - key0));
+    for (int i = lane; i < rows * chunks; i += 32) {
+      const int r = i / chunks;
+      const uint4 x = *reinterpret_cast<const uint4*>(vb + (int64_t(t.k0) + key0 + r) * a.v_stride + (i - r * chunks) * 8);
+      constexpr unsigned m = 0x7f807f80u, one = 0x00800080u;  // an exponent of all ones carries into the sign bit
+      odd |= ((((x.x & m) + one) | ((x.y & m) + one) | ((x.z & m) + one) | ((x.w & m) + one)) & 0x80008000u) != 0;
+    }
+  }
+  return __any_sync(0xffffffffu, odd);
+}
 
 // Asks the hardware for a CTA of this launch that has not started; its number, or -1 when there is none left.  The answer lands
 // in shared memory (16 bytes) and completes `bar`.
@@ -432,8 +439,6 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       mbar_init(smem_u32(&sm.q_full[i]), 1), mbar_init(smem_u32(&sm.q_empty[i]), 1), mbar_init(smem_u32(&sm.s_full[i]), 1);
       mbar_init(smem_u32(&sm.pv_done[i]), 1), mbar_init(smem_u32(&sm.p_full[i]), 4), mbar_init(smem_u32(&sm.o_empty[i]), 4);
       mbar_init(smem_u32(&sm.tile_full[i]), 1), mbar_init(smem_u32(&sm.tile_empty[i]), kReaders);
-      mbar_init(smem_u32(&sm.marks_seen[i]), 4);
-      sm.poison[i][0] = sm.poison[i][1] = 0;
     }
     mbar_init(smem_u32(&sm.s_free), 4), mbar_init(smem_u32(&sm.asked), 1), mbar_init(smem_u32(&sm.wanted), 1);
     for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
@@ -442,6 +447,10 @@ __global__ void __launch_bounds__(kThreadsW, 1)
   if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == kTmaWarp && lane < 3) {
+    const CUtensorMap* map = lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
   pdl_launch_dependents();
   fence_before();
@@ -605,7 +614,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
     const unsigned lanes = unsigned((warp & 3) * 32) << 16;
     const unsigned ts = tmem + lanes + kTmemS, tp = tmem + lanes + kTmemP + unsigned(h) * 64, to = tmem + lanes + kTmemO + unsigned(h) * 128;
     unsigned char* stage = sm.stage[h] + (warp & 3) * (32 * 128);  // 32 rows of 64 channels on their way out
-    int fill0 = 0, all = 0, used = 0, marks = 0;  // fills in front of this tile; blocks, outputs and marked outputs that the half has had
+    int all = 0;  // blocks that the half has had
     for (int n = 0;; n++) {
       // The tile stays this warp's until its output is done; what the loop over the blocks does not need is read again behind it
       // (a row of scores leaves few registers).
@@ -630,31 +639,6 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         if (!(block <= last && (block < sinks || block >= from))) continue;
         const bool edge = !(block < full_to && (block >= full_from || block < full_sinks));
         // A wait that runs out: the warp goes on without waiting for anything else.  Its lanes agree on the outcome.
-        if (edge) {
-          // V of this block, before the scores are there: zero what lies behind the sequence, look for values that are not
-          // finite in the rest (an exponent of all ones carries into the sign bit when one is added to it)
-          const int fv = fill0 + 2 * j + 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.full[fv % kSt]), unsigned(fv / kSt) & 1u));
-          uint4* vt = reinterpret_cast<uint4*>(sm.kv[fv % kSt]);
-          const int there = tile.nk - block * kN;
-          unsigned odd = 0;
-          if (ok) {
-#pragma unroll
-            for (int i = 0; i < Cfg::kTileBytes / 16 / kM; i++) {
-              const uint4 x = vt[i * kM + row_h];
-              constexpr unsigned e = 0x7f807f80u, one = 0x00800080u;
-              const unsigned y = ((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one);
-              // row of the tile: 8 chunks of 16 bytes a row, 128 rows of each 64 channels
-              if (((i * kM + row_h) >> 3) % kN < there) odd |= y;
-            }
-          }
-          if (odd & 0x80008000u) sm.poison[h][used & 1] = 1;
-          if (ok && there < kN) {
-            for (int i = row_h; i < Cfg::kTileBytes / 16; i += kM)
-              if ((i >> 3) % kN >= there) vt[i] = make_uint4(0u, 0u, 0u, 0u);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          }
-        }
         ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(all) & 1u));
         fence_after();
         unsigned s[4][32];
@@ -711,36 +695,24 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           }
         }
         const float base = m == -INFINITY ? 0.f : m * L.scale2;
-        float l4[4] = {0.f, 0.f, 0.f, 0.f};
-        // P is the product's until it has retired
-        auto wait_p = [&]() {
-          if (done > 0 && ok) {
+        const uint64_t scale2 = pair(L.scale2, L.scale2), neg_base = pair(-base, -base);
+        uint64_t l2[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned p[16];
+          exp_chunk(s[c], scale2, neg_base, l2, p);
+          if (c == 0 && done > 0 && ok) {  // P is the product's until it has retired
             ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u));
             fence_after();
           }
-        };
-        if (edge) {  // a masked score has to come out as exactly 0
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            unsigned p[16];
-            exp_chunk<false>(s[c], L.scale2, base, l4, p);
-            if (c == 0) wait_p();
-            tmem_st16(tp + 16 * c, p);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            unsigned p[16];
-            exp_chunk<true>(s[c], L.scale2, base, l4, p);
-            if (c == 0) wait_p();
-            tmem_st16(tp + 16 * c, p);
-          }
+          tmem_st16(tp + 16 * c, p);
         }
         if (ok) hand_over(&sm.p_full[h], lane);
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        float l0, l1;
+        split(add2(l2[0], l2[1]), l0, l1);
+        l += l0 + l1;
         done++, all++;
       }
-      fill0 += 2 * blocks;
       // ---- output ----
       if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u);
       ok = __all_sync(0xffffffffu, ok);
@@ -749,9 +721,11 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       const WindowTile t = tile;
       const int rh0 = t.r0 + h * kM + (warp & 3) * 32, rows_w = min(32, t.rows - (rh0 - t.r0));  // of this warp, none if negative
       const int64_t row0 = int64_t(t.q0) + rh0;
-      const bool poisoned = done > 0 && *reinterpret_cast<volatile int*>(&sm.poison[h][used & 1]);
       const bool some = l > 0.f || l != l;
       const float f = some ? 1.f / l : 0.f;
+      const uint64_t f2 = pair(f, f);
+      uint64_t odd2 = 0;  // becomes NaN with an output that is not finite
+      mxk_bf16* dst = a.out + (row0 + (lane >> 3)) * a.out_stride + int64_t(t.head) * a.D + 8 * (lane & 7);
 #pragma unroll 1
       for (int c = 0; c < DP / 64; c++) {
         unsigned o[2][32];
@@ -773,38 +747,41 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         // chunks of a row exchanged by the row's number.
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          float x[8];
+          unsigned w[4];
 #pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = __uint_as_float(o[i >> 2][8 * (i & 3) + e]) * f;  // 0 * 0 in a row that sees nothing
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) = pack8(x);
-        }
-        __syncwarp();
-        if (!poisoned) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int r = 4 * i + (lane >> 3), ch = 64 * c + 8 * (lane & 7);
-            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
-            if (r < rows_w && ch < a.D) *reinterpret_cast<uint4*>(a.out + (row0 + r) * a.out_stride + int64_t(t.head) * a.D + ch) = x;
+          for (int e = 0; e < 4; e++) {
+            const int k = 8 * (i & 3) + 2 * e;
+            const uint64_t x = fma2(pair(__uint_as_float(o[i >> 2][k]), __uint_as_float(o[i >> 2][k + 1])), f2, 0);  // 0 * 0 in a row that sees nothing
+            odd2 = fma2(x, 0, odd2);
+            float lo, hi;
+            split(x, lo, hi);
+            w[e] = pack_bf16(lo, hi);
           }
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int r = 4 * i + (lane >> 3);
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) * 16));
+          if (r < rows_w && 64 * c + 8 * (lane & 7) < a.D) *reinterpret_cast<uint4*>(dst + 4 * i * a.out_stride + 64 * c) = x;
         }
         __syncwarp();
       }
-      if (!poisoned && a.lse && lane < rows_w)
+      if (a.lse && lane < rows_w)
         a.lse[(row0 + lane) * a.H + t.head] = some ? (m == -INFINITY ? 0.f : m * L.scale2 * kLn2) + log2f(l) * kLn2 : -INFINITY;
-      if (poisoned) {
-        for (int r = 0; r < rows_w; r++)
+      // An output that is not finite although the row's scores are: a value that the row sees, or one of a block that it does
+      // not see all of, which has come in as 0 * v.  Where there is such a value, the row is taken again without it.
+      float odd, odd_hi;
+      split(odd2, odd, odd_hi);
+      odd += odd_hi;
+      unsigned again = __ballot_sync(0xffffffffu, odd != odd && l == l && lane < rows_w);
+      if (again && hidden_value_odd(L, t, h)) {
+        for (; again; again &= again - 1) {
+          const int r = __ffs(again) - 1;
           row_attention(L, row0 + r, t.head, t.k0, rh0 + r + t.nk - t.nq, t.nk, reinterpret_cast<float*>(stage));
-        // The mark is taken back once the half's four warps have seen it.  Nobody sets it again before: that takes another
-        // tile's product with V in between, which needs the probabilities of all four.
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(smem_u32(&sm.marks_seen[h]));
-        if ((warp & 3) == 0) {
-          ok = wait(&sm.marks_seen[h], marks);
-          if (lane == 0) sm.poison[h][used & 1] = 0;
         }
-        marks++;
       }
-      if (done > 0) used++;
       __syncwarp();
       if (lane == 0) mbar_arrive1(smem_u32(&sm.tile_empty[n & 1]));
     }
