@@ -38,11 +38,7 @@ __all__ = [
 
 
 def _p(t) -> Optional[int]:
-    if t is None:
-        return None
-    if isinstance(t, int):
-        return t
-    return t.data_ptr()
+    return t if t is None or t.__class__ is int else t.data_ptr()
 
 
 # The current stream's handle without a Stream object around it (0.3 instead of 3.2 us per call, which is most of what a
@@ -368,10 +364,15 @@ class KvCache:
                                  k.shape[2], k.shape[3], KV_BF16 if k.dtype == torch.bfloat16 else KV_E4M3)
 
 
-def _here(what, index):
-    """The library works on the current device; a tensor of another one is refused before its address gets there."""
-    if index >= 0 and index != torch.cuda.current_device():
-        raise MxkError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+def _here(what, index, stream=None):
+    """The library works on the current device; a tensor of another one (of index `index`, -1: none) is refused before its
+    address gets there.  Returns the handle of the stream the call goes to."""
+    now = torch.cuda.current_device()
+    if index >= 0 and index != now:
+        raise MxkError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{now}")
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(now) or None
+    return _stream(stream)
 
 
 def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, table_rows, rot, mode, cache: KvCache, positions,
@@ -380,12 +381,12 @@ def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, ta
     c = cache._args
     if D != c.D:
         raise MxkError(f"qkv_norm_rope_append: D={D} and a cache of D={c.D}")
-    _here("qkv_norm_rope_append", cache._index)
+    handle = _here("qkv_norm_rope_append", cache._index, stream)
     kv = c.Hkv * D
     a = AppendArgs(_p(q), _p(k), _p(v), T, H * D if q_stride is None else q_stride, kv if k_stride is None else k_stride,
                    kv if v_stride is None else v_stride, _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), table_rows, _p(positions),
                    _p(seq_ids), _p(rope_rows), _p(q_out), _p(k_out), H, rot, mode, eps)
-    check(lib().mxk_qkv_norm_rope_append(a, c, _stream(stream)))
+    check(lib().mxk_qkv_norm_rope_append(a, c, handle))
 
 
 def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
@@ -401,9 +402,9 @@ def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
 def attn_decode_paged(q, cache: KvCache, seq_lens, H, scale, out, left=-1, sinks=0, q_stride=None, lse=None, *, workspace, stream=None):
     """Attention of one new token of every sequence over its tokens in the cache."""
     c = cache._args
-    _here("attn_decode_paged", cache._index)
+    handle = _here("attn_decode_paged", cache._index, stream)
     a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), left, sinks, H, scale)
-    check(lib().mxk_attn_decode_paged(a, c, _stream(stream)))
+    check(lib().mxk_attn_decode_paged(a, c, handle))
 
 
 def attn_window(q, k, v, q_rows, k_rows, H, Hkv, D, scale, out, left=-1, right=-1, sinks=0, cu_q=None, cu_k=None, n_seqs=None,
@@ -412,12 +413,11 @@ def attn_window(q, k, v, q_rows, k_rows, H, Hkv, D, scale, out, left=-1, right=-
     window of `left` / `right` keys (-1: no bound; right = 0: causal) and `sinks` first keys that stay visible."""
     if n_seqs is None:
         n_seqs = 1 if cu_q is None else cu_q.numel() - 1
-    if not isinstance(q, int):
-        _here("attn_window", q.get_device())
+    handle = _here("attn_window", -1 if q.__class__ is int else q.get_device(), stream)
     a = AttnArgs(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k), q_rows, k_rows, H * D if q_stride is None else q_stride,
                  Hkv * D if k_stride is None else k_stride, Hkv * D if v_stride is None else v_stride,
                  H * D if out_stride is None else out_stride, left, right, sinks, n_seqs, H, Hkv, D, scale)
-    check(lib().mxk_attn_window(a, _stream(stream)))
+    check(lib().mxk_attn_window(a, handle))
 
 
 def _qmat_for(x, rows, dim, out):
