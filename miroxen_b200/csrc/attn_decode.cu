@@ -16,7 +16,7 @@
 // sum and unnormalised output in its slots of the workspace (one for the segment its run starts in, one for the segment
 // it ends in) and join_kernel, launched behind it, adds them up in order.  Results do not depend on timing.
 //
-// Within a CTA a fifth warp brings the tiles of K and V into a ring of shared-memory stages (16-byte cp.async, rows found
+// Within a CTA two warps bring the tiles of K and V into a ring of shared-memory stages (16-byte cp.async, rows found
 // through the page table one tile ahead, completion counted on mbarriers) and four warps do the arithmetic.  For the scores
 // each takes a quarter of the tile's tokens; for the product with V each takes a quarter of the channels of all tokens, so
 // that the output stays in a few registers and only the probabilities pass through shared memory.  They are taken relative
@@ -35,8 +35,9 @@
 namespace mxk {
 namespace {
 
-constexpr int kWarps = 4;       // that compute; one more copies
-constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32;
+constexpr int kWarps = 4;       // that compute
+constexpr int kCopyWarps = 2;   // that copy, 32 tokens of a tile each
+constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32 * kCopyWarps;
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -201,6 +202,7 @@ template <bool E4M3, int DP>
 struct DecodeCfg {
   static constexpr int kTokW = 16;  // tokens per warp
   static constexpr int kTile = kTokW * kWarps;
+  static_assert(kTile == 32 * kCopyWarps, "a copying warp looks up a token per lane");
   static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2), kPitch = kRowBytes + 16;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kTileBytes = kTile * kPitch;
@@ -226,8 +228,8 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   const unsigned ring_u = smem_u32(ring);
   pdl_launch_dependents();
   if (tid == 0) {
-    // a stage is full when the copies of the copying warp's 32 threads have landed and its word on the tokens is written
-    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&full[i]), 33), mbar_init(smem_u32(&empty[i]), kWarps);
+    // a stage is full when the copies of the copying warps' threads have landed and their words on the tokens are written
+    for (int i = 0; i < kSt; i++) mbar_init(smem_u32(&full[i]), 33 * kCopyWarps), mbar_init(smem_u32(&empty[i]), kWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (D < DP) {  // channels [D, DP) of every row stay zero (the copies never touch them)
@@ -254,65 +256,55 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   cur.head = (t0 - before) / cur.n_tiles, cur.tile = (t0 - before) % cur.n_tiles;
   bool ok = true;
 
-  if (warp == kWarps) {
-    // ---- the copying warp ----
-    constexpr int kPerInstr = 32 / Cfg::kChunks, kWords = kTile / 32;  // rows per instruction; tokens a lane looks up
-    const int ch = lane % Cfg::kChunks, sub = lane / Cfg::kChunks;
+  if (warp >= kWarps) {
+    // ---- the copying warps ----
+    constexpr int kPerInstr = 32 / Cfg::kChunks;  // rows per instruction
+    const int ch = lane % Cfg::kChunks, sub = lane / Cfg::kChunks, part = warp - kWarps;
     const bool copies = ch * 16 < D * int(sizeof(elem));
-    const unsigned char *kb = static_cast<const unsigned char*>(p.c.k) + ch * 16, *vb = static_cast<const unsigned char*>(p.c.v) + ch * 16;
-    // Pages and slots of tokens lane, lane + 32, ... of the tile that is copied next (slot -1: no token), asked for before the
-    // tile in front of it is copied and not looked at until then, so that the page table's latency passes meanwhile.
-    int page[kWords], slot[kWords];
+    const unsigned char* kb = static_cast<const unsigned char*>(p.c.k) + ch * 16;
+    const int64_t to_v = static_cast<const unsigned char*>(p.c.v) - static_cast<const unsigned char*>(p.c.k);
+    // Page and slot of token 32 part + lane of the tile that is copied next (slot -1: no token), asked for before the tile in
+    // front of it is copied and not looked at until then, so that the page table's latency passes meanwhile.
+    int page, slot;
     int64_t head_off;
     auto look_up = [&]() {
       head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
-#pragma unroll
-      for (int u = 0; u < kWords; u++) {
-        const int i = cur.tile * kTile + u * 32 + lane;
-        page[u] = 0, slot[u] = -1;
-        if (i < cur.v.len) {  // inside the table: the length is held to it
-          const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
-          // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
-          int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
-          if (r >= p.c.page_size) n++, r -= p.c.page_size;
-          slot[u] = r;
-          page[u] = p.c.page_table[int64_t(cur.b) * p.c.table_stride + n];
-        }
+      const int i = cur.tile * kTile + part * 32 + lane;
+      page = 0, slot = -1;
+      if (i < cur.v.len) {  // inside the table: the length is held to it
+        const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
+        // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
+        int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
+        if (r >= p.c.page_size) n++, r -= p.c.page_size;
+        slot = r;
+        page = p.c.page_table[int64_t(cur.b) * p.c.table_stride + n];
       }
       cursor_next<kTile>(p, cur);
     };
     look_up();
     int st = 0;
     for (int i = 0; i < n_my; i++) {
-      int64_t off[kWords];  // byte offsets, -1: not there
-#pragma unroll
-      for (int u = 0; u < kWords; u++) {
-        off[u] = -1;
-        if (slot[u] >= 0) {
-          if (page[u] >= 0 && page[u] < p.c.num_pages) off[u] = (int64_t(page[u]) * p.c.page_stride + int64_t(slot[u]) * p.c.token_stride + head_off) * int(sizeof(elem));
-          else if (p.err) atomicExch(p.err, kErrBadIndex);
-        }
+      int64_t off = -1;  // byte offset, -1: not there
+      if (slot >= 0) {
+        if (page >= 0 && page < p.c.num_pages) off = (int64_t(page) * p.c.page_stride + int64_t(slot) * p.c.token_stride + head_off) * int(sizeof(elem));
+        else if (p.err) atomicExch(p.err, kErrBadIndex);
       }
       if (i + 1 < n_my) look_up();
       if (i >= kSt) {
         ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u));
         if (!ok) break;
       }
-      const unsigned dk = ring_u + unsigned(st) * 2 * Cfg::kTileBytes + unsigned(sub * kPitch + ch * 16);
+      const unsigned dk = ring_u + unsigned(st) * 2 * Cfg::kTileBytes + unsigned((part * 32 + sub) * kPitch + ch * 16);
+      const unsigned word = __ballot_sync(0xffffffffu, off >= 0);
+      if (lane == 0) there[st][part] = word;
 #pragma unroll
-      for (int u = 0; u < kWords; u++) {
-        const unsigned word = __ballot_sync(0xffffffffu, off[u] >= 0);
-        if (lane == 0) there[st][u] = word;
-#pragma unroll
-        for (int r = 0; r < 32 / kPerInstr; r++) {
-          const int row = u * 32 + r * kPerInstr;  // + sub
-          const int64_t o = __shfl_sync(0xffffffffu, off[u], r * kPerInstr + sub);
-          if (copies) {  // a token that is not there reads as zeros: its value must not carry anything into 0 * v
-            const unsigned n = o >= 0 ? 16u : 0u;
-            const int64_t x = o >= 0 ? o : 0;
-            cp_async16(dk + unsigned(row * kPitch), kb + x, n);
-            cp_async16(dk + unsigned(Cfg::kTileBytes + row * kPitch), vb + x, n);
-          }
+      for (int r = 0; r < 32 / kPerInstr; r++) {
+        const int64_t o = __shfl_sync(0xffffffffu, off, r * kPerInstr + sub);
+        if (copies) {  // a token that is not there reads as zeros: its value must not carry anything into 0 * v
+          const unsigned n = o >= 0 ? 16u : 0u;
+          const unsigned char* x = kb + (o >= 0 ? o : 0);
+          cp_async16(dk + unsigned(r * kPerInstr * kPitch), x, n);
+          cp_async16(dk + unsigned(Cfg::kTileBytes + r * kPerInstr * kPitch), x + to_v, n);
         }
       }
       cp_async_arrive(smem_u32(&full[st]));
