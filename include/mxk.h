@@ -244,7 +244,7 @@ int mxk_linear_gated_residual(const mxk_bf16* A, const mxk_bf16* W, const float*
  * page_table[b * table_stride + t / page_size]; a sequence has room for max_pages * page_size tokens.  The same page
  * may stand in several rows of the table (a shared prefix).
  * type MXK_KV_BF16: bf16 values.  MXK_KV_E4M3: fp8 e4m3 values, element = value / scale rounded to nearest, ties to
- * even, saturating at +-448; k_scale / v_scale fp32 [Hkv] or NULL (1).
+ * even, saturating at +-448; k_scale / v_scale fp32 [Hkv], positive normal numbers, or NULL (1).
  * Page numbers, sequence numbers, positions and lengths are read on the device.  One that is out of range is never
  * followed: the row or token is left out and mxk_device_error() reports MXK_DEVICE_ERR_BAD_INDEX. */
 #define MXK_KV_BF16 0
@@ -297,8 +297,8 @@ int mxk_qkv_norm_rope_append(const MxkAppendArgs* args_host, const MxkKvCache* c
  * receives the natural logarithm of the softmax's denominator.  A sequence of length 0 gives out 0 and lse -inf.
  * The work is split evenly over the GPU along the cached tokens and joined by a second launch through `workspace`
  * (mxk_attn_decode_workspace_bytes(cache, H) bytes of device memory, 16-byte aligned, no initial value; calls that may
- * run at the same time, two captured graphs among them, need one each).  H a multiple of Hkv; D a multiple of 8 (16
- * for e4m3), at most 128. */
+ * run at the same time, two captured graphs among them, need one each; asked for on the device that the call is made
+ * on).  H a multiple of Hkv; D a multiple of 8 (16 for e4m3), at most 128; 0 < scale <= 1e30; out overlaps no input. */
 typedef struct MxkDecodeArgs {
   const mxk_bf16* q;
   int64_t q_stride;
@@ -306,7 +306,7 @@ typedef struct MxkDecodeArgs {
   mxk_bf16* out;
   float* lse;
   void* workspace;
-  int64_t left, sinks;
+  int64_t workspace_bytes, left, sinks;
   int32_t H;
   float scale;
 } MxkDecodeArgs;
@@ -323,7 +323,8 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args_host, const MxkKvCache* cach
  * nothing gives out 0 and lse -inf; rows of q and out that belong to no sequence are left as they were, and k / v rows
  * that belong to no sequence, or lie outside of every row's view, do not reach any output whatever they hold.
  * q, k, v, out: bf16, head h of a row at row * stride + h * D; strides multiples of 8, pointers 16-byte aligned;
- * head h reads key head h / (H / Hkv); D a multiple of 8, at most 128.  out overlaps no input. */
+ * head h reads key head h / (H / Hkv); D a multiple of 8, at most 128; fewer than 2^30 rows; 0 < scale <= 1e30.  out
+ * overlaps no input. */
 typedef struct MxkAttnArgs {
   const mxk_bf16* q;
   const mxk_bf16* k;

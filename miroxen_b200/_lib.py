@@ -67,7 +67,7 @@ class AppendArgs(C.Structure):
 class DecodeArgs(C.Structure):
     """MxkDecodeArgs."""
     _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("seq_lens", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
-                ("workspace", C.c_void_p), ("left", C.c_int64), ("sinks", C.c_int64), ("H", C.c_int32), ("scale", C.c_float)]
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("left", C.c_int64), ("sinks", C.c_int64), ("H", C.c_int32), ("scale", C.c_float)]
 
 
 class AttnArgs(C.Structure):

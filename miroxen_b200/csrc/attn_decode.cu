@@ -666,6 +666,10 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   // no more runs than there can be tiles
   const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, kTile);
   if (p.ctas > most) p.ctas = int(most < 1 ? 1 : most);
+  const int64_t need = int64_t(2) * p.ctas * kRows * (DP + 2) * int64_t(sizeof(float));
+  if (p.a.workspace_bytes < need)
+    return fail(MXK_ERR_INVALID_ARG, "%s: workspace of %lld bytes, mxk_attn_decode_workspace_bytes() asks for up to %lld", name, (long long)p.a.workspace_bytes,
+                (long long)need);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
   launch_pdl(decode_kernel<E4M3, DP, NH>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
@@ -723,7 +727,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(static_cast<const char*>(a.workspace), 16))
     return fail(MXK_ERR_INVALID_ARG, "%s: q, out and workspace must be 16-byte aligned", name);
   if (a.sinks < 0) return fail(MXK_ERR_INVALID_ARG, "%s: sinks=%lld", name, (long long)a.sinks);
-  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and finite", name);
+  if (!(a.scale > 0.f) || a.scale > 1e30f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and at most 1e30", name);
   p.group = a.H / cache->Hkv;
   p.blocks = int(ceil_div(p.group, 16));
   p.heads = cache->Hkv * p.blocks;

@@ -288,32 +288,37 @@ struct WindowTile {
   int q0, nq, k0, nk, r0, rows, head;
 };
 
-// Tile number `cta` of the launch, by one warp; rows = 0 if there is no such tile.  The tiles at the end of a causal sequence,
-// which have the most keys, come first, all heads of a tile one behind the other: the other way round, head by head, the CTAs
-// at work crowd on the same few lines of the keys (packed prompts XX against YY us).
-__device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta) {
+// Where a warp's search for tiles has got to: `seqs` sequences from the back with `tiles` tiles.
+struct TileSearch {
+  int seqs = 0, tiles = 0;
+};
+
+// Tile number `cta` of the launch, by one warp; rows = 0 if there is no such tile.  Counted from the back: the tiles at the end
+// of a causal sequence, which have the most keys, come first, all heads of a tile one behind the other (the other way round,
+// head by head, the CTAs at work crowd on the same few lines of the keys: packed prompts 195 against 145 us).  Numbers never
+// fall from one search of a CTA to its next, so that each goes on where the last one ended.
+__device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta, TileSearch& from) {
   const MxkAttnArgs& a = W.L.a;
-  const int lane = threadIdx.x & 31, tile_rows = kM * W.halves;
-  const int place = cta / a.H, want = W.max_tiles - 1 - place;
+  const int lane = threadIdx.x & 31, tile_rows = kM * W.halves, place = cta / a.H;
   WindowTile t{0, int(a.q_rows), 0, int(a.k_rows), 0, 0, cta - place * a.H};
   if (!a.cu_q) {
-    t.r0 = want * tile_rows;
+    t.r0 = (W.max_tiles - 1 - place) * tile_rows;
     t.rows = min(tile_rows, t.nq - t.r0);
     return t;
   }
   constexpr int kAhead = 4;  // groups of 32 sequences whose ends are asked for at once
-  int at = 0;                // tiles of the sequences in front
-  for (int base = 0; base < a.n_seqs; base += 32 * kAhead) {
+  for (; from.seqs < a.n_seqs; from.seqs += 32 * kAhead) {
     int x[kAhead][4];
 #pragma unroll
     for (int u = 0; u < kAhead; u++) {
-      const int b = base + 32 * u + lane;
+      const int b = a.n_seqs - 1 - (from.seqs + 32 * u + lane);
       x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0;
-      if (b < a.n_seqs) x[u][0] = a.cu_q[b], x[u][1] = a.cu_q[b + 1], x[u][2] = a.cu_k[b], x[u][3] = a.cu_k[b + 1];
+      if (b >= 0) x[u][0] = a.cu_q[b], x[u][1] = a.cu_q[b + 1], x[u][2] = a.cu_k[b], x[u][3] = a.cu_k[b + 1];
     }
+    int at = from.tiles;
 #pragma unroll
     for (int u = 0; u < kAhead; u++) {
-      if (base + 32 * u >= a.n_seqs) break;
+      if (from.seqs + 32 * u >= a.n_seqs) break;
       // held inside the arrays and in order whatever they hold
       const int q0 = max(0, min(x[u][0], int(a.q_rows))), q1 = max(q0, min(x[u][1], int(a.q_rows)));
       const int k0 = max(0, min(x[u][2], int(a.k_rows))), k1 = max(k0, min(x[u][3], int(a.k_rows)));
@@ -326,17 +331,18 @@ __device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta) 
         if (lane >= o) incl += y;
       }
       const int first = at + incl - mine;
-      const unsigned hit = __ballot_sync(0xffffffffu, want >= first && want < first + mine);
+      const unsigned hit = __ballot_sync(0xffffffffu, place >= first && place < first + mine);
       if (hit) {
         const int src = __ffs(hit) - 1;
         t.q0 = __shfl_sync(0xffffffffu, q0, src), t.nq = __shfl_sync(0xffffffffu, q1 - q0, src);
         t.k0 = __shfl_sync(0xffffffffu, k0, src), t.nk = __shfl_sync(0xffffffffu, k1 - k0, src);
-        t.r0 = (want - __shfl_sync(0xffffffffu, first, src)) * tile_rows;
+        t.r0 = __shfl_sync(0xffffffffu, mine - 1 - (place - first), src) * tile_rows;
         t.rows = min(tile_rows, t.nq - t.r0);
         return t;
       }
       at += __shfl_sync(0xffffffffu, incl, 31);
     }
+    from.tiles = at;
   }
   return t;
 }
@@ -485,8 +491,9 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       // ---- which tiles: this CTA's own, then those of CTAs that have not started yet.  One is asked for when the loads of
       // the tile at hand come to their end, no earlier: what a CTA has asked for no other can take at the end of the launch.
       int cta = int(blockIdx.x), n = 0;
+      TileSearch search;
       for (int asks = 0; ok; asks++) {
-        t = find_tile(W, cta);
+        t = find_tile(W, cta, search);
         if (t.rows > 0) {
           if (n >= 2) ok = wait(&sm.tile_empty[n & 1], (n >> 1) - 1);
           if (ok && leader) {
@@ -870,7 +877,7 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   if (a.q_rows <= 0 || a.n_seqs <= 0) return MXK_OK;
   if (!a.q || !a.out) return fail(MXK_ERR_INVALID_ARG, "%s: null q or out", name);
   if (a.k_rows < 0 || (a.k_rows > 0 && (!a.k || !a.v))) return fail(MXK_ERR_INVALID_ARG, "%s: k_rows=%lld, null k or v", name, (long long)a.k_rows);
-  if (a.H <= 0 || a.Hkv <= 0 || a.H % a.Hkv != 0 || a.H > 65535)
+  if (a.H <= 0 || a.Hkv <= 0 || a.H % a.Hkv != 0)
     return fail(MXK_ERR_INVALID_ARG, "%s: H=%d must be a positive multiple of Hkv=%d", name, a.H, a.Hkv);
   if (a.D < 8 || a.D > MXK_ATTN_MAX_HEAD_DIM || a.D % 8 != 0)
     return fail(MXK_ERR_INVALID_ARG, "%s: head dimension %d must be a multiple of 8 and at most %d", name, a.D, MXK_ATTN_MAX_HEAD_DIM);
@@ -886,7 +893,7 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16))
     return fail(MXK_ERR_INVALID_ARG, "%s: q, k, v and out must be 16-byte aligned", name);
   if (a.sinks < 0) return fail(MXK_ERR_INVALID_ARG, "%s: sinks=%lld", name, (long long)a.sinks);
-  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and finite", name);
+  if (!(a.scale > 0.f) || a.scale > 1e30f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and at most 1e30", name);
   L.group = a.H / a.Hkv;
   L.scale2 = a.scale * kLog2e;
   L.err = device_error_word();

@@ -390,8 +390,8 @@ def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, ta
 
 
 def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
-    """Scratch memory for attn_decode_paged with this cache and head count: keep one for each stream or graph that may
-    run at the same time as another."""
+    """Scratch memory for attn_decode_paged with this cache and head count, allocated on the current stream: keep one for
+    each stream or graph that may run at the same time as another."""
     _here("attn_decode_workspace", cache._index)
     n = lib().mxk_attn_decode_workspace_bytes(cache._args, H)
     if n < 0:
@@ -403,7 +403,7 @@ def attn_decode_paged(q, cache: KvCache, seq_lens, H, scale, out, left=-1, sinks
     """Attention of one new token of every sequence over its tokens in the cache."""
     c = cache._args
     handle = _here("attn_decode_paged", cache._index, stream)
-    a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), left, sinks, H, scale)
+    a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), workspace.nbytes, left, sinks, H, scale)
     check(lib().mxk_attn_decode_paged(a, c, handle))
 
 

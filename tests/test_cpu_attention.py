@@ -31,7 +31,7 @@ def append(L, **more):
 
 
 def decode(L, **more):
-    a = L.DecodeArgs(P, 32 * 128, P, P, P, P, -1, 0, 32, 0.1)
+    a = L.DecodeArgs(P, 32 * 128, P, P, P, P, 1 << 40, -1, 0, 32, 0.1)
     for k, v in more.items():
         setattr(a, k, v)
     return a
@@ -93,8 +93,8 @@ def test_append_null_structs_and_noops(L):
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(seq_lens=None), dict(out=None), dict(workspace=None), dict(q=P + 2), dict(out=P + 8),
-                                 dict(workspace=P + 4), dict(q_stride=12), dict(q_stride=-8), dict(sinks=-1), dict(scale=0.0),
-                                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(H=0), dict(H=12)], ids=str)
+                                 dict(workspace=P + 4), dict(workspace_bytes=4096), dict(workspace_bytes=-1), dict(q_stride=12), dict(q_stride=-8), dict(sinks=-1), dict(scale=0.0),
+                                 dict(scale=-1.0), dict(scale=2e30), dict(scale=float("nan")), dict(scale=float("inf")), dict(H=0), dict(H=12)], ids=str)
 def test_decode_refusals(L, bad):
     lib = L.lib()
     assert lib.mxk_attn_decode_paged(decode(L, **bad), cache(L), None) == -1
@@ -124,7 +124,7 @@ def test_window_refusals(L, bad):
 def test_window_sizes_and_noops(L):
     lib = L.lib()
     assert lib.mxk_attn_window(None, None) == -1
-    assert lib.mxk_attn_window(window(L, q_rows=1 << 31), None) == -3
+    assert lib.mxk_attn_window(window(L, q_rows=1 << 30), None) == -3
     assert lib.mxk_attn_window(window(L, k_rows=1 << 31), None) == -3
     assert lib.mxk_attn_window(window(L, q_rows=0, q=None), None) == 0
     assert lib.mxk_attn_window(window(L, q_rows=-5), None) == 0
@@ -134,7 +134,7 @@ def test_window_sizes_and_noops(L):
 def test_struct_sizes_match_the_header(L):
     assert C.sizeof(L.KvCacheArgs) == 5 * 8 + 5 * 8 + 6 * 4
     assert C.sizeof(L.AppendArgs) == 3 * 8 + 4 * 8 + 4 * 8 + 8 + 5 * 8 + 4 * 4
-    assert C.sizeof(L.DecodeArgs) == 6 * 8 + 2 * 8 + 2 * 4
+    assert C.sizeof(L.DecodeArgs) == 6 * 8 + 3 * 8 + 2 * 4
     assert C.sizeof(L.AttnArgs) == 7 * 8 + 9 * 8 + 4 * 4 + 8
 
 

@@ -340,6 +340,17 @@ def test_decode_bad_pages_and_lengths_are_left_out_and_reported(mx):
     assert bool((out[3] == 0).all()) and torch.equal(out[0], good[0])
 
 
+def test_decode_refuses_a_small_workspace(mx):
+    g = gen(24)
+    cache = make_cache(mx, g, BF16, 2, 4000, 16, 2, 128)
+    q, out = rand(g, 2, 8, 128), torch.full((2, 8, 128), 7.0, device="cuda", dtype=torch.bfloat16)
+    sl = torch.tensor([4000, 100], device="cuda", dtype=torch.int32)
+    with pytest.raises(mx.MxkError, match="workspace"):
+        mx.attn_decode_paged(q, cache, sl, 8, 0.09, out, workspace=mx.attn_decode_workspace(cache, 8)[:4096])
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
+
+
 def test_decode_offsets_past_32_bits(mx):
     g = gen(21)
     pages, page, Hkv, D = 18000, 128, 8, 128  # 2.36e9 elements each
@@ -438,6 +449,15 @@ def test_window_many_sequences(mx):
     rng = random.Random(8)
     rows = [rng.choice([0, 1, 2, rng.randrange(1, 200)]) for _ in range(150)]
     check_window(mx, 35, rows, [n + rng.randrange(0, 30) for n in rows], 2, 1, 64, -1, 0, 0)
+
+
+def test_window_thousands_of_sequences(mx):
+    """More sequences than a search looks at at once, most of them empty or of one row."""
+    rng = random.Random(9)
+    rows = [rng.choice([0, 0, 1, 1, 2, 5]) for _ in range(1500)]
+    rows[3], rows[700], rows[1499] = 300, 129, 257
+    check_window(mx, 36, rows, [n + (i % 3 if n else 0) for i, n in enumerate(rows)], 1, 1, 64, -1, 0, 0)
+    check_window(mx, 36, [1] * 700, [1] * 700, 2, 1, 128, 3, 0, 1, behind=5)
 
 
 def test_window_scores_that_grow_along_the_keys(mx):
