@@ -14,7 +14,9 @@
 // end inside a sequence's tokens and cover several short sequences.  Each CTA finds the run's start itself by summing the
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
 // sum and unnormalised output in its slots of the workspace (one for the segment its run starts in, one for the segment
-// it ends in) and join_kernel, launched behind it, adds them up in order.  Results do not depend on timing.
+// it ends in) and join_kernel, launched behind it, adds them up in order.  Where the whole call is short, that second launch is
+// most of it: if all work items cut into at most 8 fit the GPU at once with at most kShort tiles for each CTA, the CTAs of an item are
+// a cluster and add up through each other's shared memory.  Results do not depend on timing.
 //
 // Within a CTA two warps bring the tiles of K and V into a ring of shared-memory stages (16-byte cp.async, rows found
 // through the page table one tile ahead, completion counted on mbarriers) and four warps do the arithmetic.  For the scores
@@ -38,6 +40,7 @@ namespace {
 constexpr int kWarps = 4;       // that compute
 constexpr int kCopyWarps = 2;   // that copy, 32 tokens of a tile each
 constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32 * kCopyWarps;
+constexpr int kShort = 8;       // tiles of a CTA up to which a call takes the form without a second launch
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -48,6 +51,7 @@ struct DecodeLaunch {
   int blocks;      // blocks of 8 or 16 of those
   int heads;       // Hkv * blocks: work items per sequence
   int ctas;        // runs
+  int cluster;     // 0: runs over all tiles; n > 0: the tiles of a work item cut among n CTAs (a cluster where n > 1)
   float scale2;    // scale * log2(e)
   unsigned page_recip;  // floor((2^32 - 1) / page_size)
   float* part_o;   // [2 ctas][rows][DP], rows: query heads per block
@@ -154,6 +158,22 @@ __device__ __forceinline__ void cp_async_arrive(unsigned bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// The cluster's threads that are still there; what they wrote to shared memory is visible to the others.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What stands at this shared-memory address in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster(unsigned addr, unsigned rank) {
+  float v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ld_cluster2(unsigned addr, unsigned rank, float& x, float& y) {
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+               : "=f"(x), "=f"(y)
+               : "r"(addr), "r"(rank)
+               : "memory");
+}
 // Barrier of the computing warps; `vote`: whether any of them has v set.
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
 __device__ __forceinline__ bool vote(bool v) {
@@ -237,10 +257,26 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   }
   pdl_wait();
 
-  int total, seq0, before;
-  int per = 0;
-  locate<kTile>(p, red, [&](int t) { return int(blockIdx.x) * (per = (t + p.ctas - 1) / p.ctas); }, total, seq0, before);
-  const int t0 = min(total, int(blockIdx.x) * per), n_my = min(total, t0 + per) - t0;
+  Cursor cur;
+  int n_my;  // tiles of this CTA's run, which starts at the cursor
+  if (p.cluster == 0) {
+    int total, before, per = 0;
+    locate<kTile>(p, red, [&](int t) { return int(blockIdx.x) * (per = (t + p.ctas - 1) / p.ctas); }, total, cur.b, before);
+    const int t0 = min(total, int(blockIdx.x) * per);
+    n_my = min(total, t0 + per) - t0;
+    if (n_my > 0) {
+      cursor_sequence<kTile>(p, cur);
+      cur.head = (t0 - before) / cur.n_tiles, cur.tile = (t0 - before) % cur.n_tiles;
+    }
+  } else {
+    const int item = int(blockIdx.x) / p.cluster, rank = int(blockIdx.x) - item * p.cluster;
+    cur.b = item / p.heads, cur.head = item - cur.b * p.heads;
+    cur.v = view_of(p, cur.b);
+    cur.n_tiles = (cur.v.len + kTile - 1) / kTile;
+    cur.tile = rank * cur.n_tiles / p.cluster;
+    n_my = (rank + 1) * cur.n_tiles / p.cluster - cur.tile;
+    __syncthreads();  // barriers and zeroed channels are there
+  }
   // sequences that have no token in view: out 0, lse -inf
   for (int b = blockIdx.x; b < p.c.n_seqs; b += gridDim.x) {
     if (view_of(p, b).len > 0) continue;
@@ -248,12 +284,9 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     if (p.a.lse)
       for (int i = tid; i < p.a.H; i += kThreadsD) p.a.lse[int64_t(b) * p.a.H + i] = -INFINITY;
   }
-  if (n_my <= 0) return;
+  const bool joins = p.cluster > 1 && cur.n_tiles > 0;  // the same for the whole cluster
+  if (n_my <= 0 && (!joins || warp >= kWarps)) return;
 
-  Cursor cur;
-  cur.b = seq0;
-  cursor_sequence<kTile>(p, cur);
-  cur.head = (t0 - before) / cur.n_tiles, cur.tile = (t0 - before) % cur.n_tiles;
   bool ok = true;
 
   if (warp >= kWarps) {
@@ -324,6 +357,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   float base[NH][2], l[NH][2], scale[NH][2];  // maximum in use (in units of log2), this thread's part of the sum, of the columns
   unsigned qf[NH][kKSteps][2];
   const int r0 = lane >> 2, c2 = lane & 3;
+  const Cursor start = cur;
   bool fresh = true;
   int first_tile = 0, st = 0, g = 0, rows = 0, h0 = 0;
   unsigned ph = 0;
@@ -527,7 +561,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
 
     const bool last = cur.tile + 1 == cur.n_tiles;
     if (last || i + 1 == n_my) {  // the (sequence, head) or the run ends: store
-      const bool whole = last && first_tile == 0;
+      const bool whole = last && first_tile == 0 && !joins;
 #pragma unroll
       for (int nh = 0; nh < NH; nh++)
 #pragma unroll
@@ -539,6 +573,9 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       meet();
       const float vs = E4M3 && p.c.v_scale ? p.c.v_scale[g] : 1.f;
       const int64_t slot = 2 * int64_t(blockIdx.x) + (first_tile == 0 ? 1 : 0);
+      // this part's place: a slot of the workspace, or this CTA's own stages, which nobody reads any more
+      float* part_o = joins ? reinterpret_cast<float*>(ring) : p.part_o + slot * kRows * DP;
+      float* part_ml = joins ? part_o + kRows * DP : p.part_ml + slot * kRows * 2;
 #pragma unroll
       for (int nh = 0; nh < NH; nh++)
 #pragma unroll
@@ -560,13 +597,12 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
               if (d0 < D) dst[d0] = mxk_bf16(w & 0xffffu);
               if (d1 < D) dst[d1] = mxk_bf16(w >> 16);
             } else {
-              float* dst = p.part_o + (slot * kRows + r) * DP;
-              dst[d0] = v0, dst[d1] = v1;
+              part_o[r * DP + d0] = v0, part_o[r * DP + d1] = v1;
             }
           }
           if (warp == 0 && r0 == 0) {
             if (!whole) {
-              p.part_ml[(slot * kRows + r) * 2] = base[nh][c], p.part_ml[(slot * kRows + r) * 2 + 1] = sum;
+              part_ml[2 * r] = base[nh][c], part_ml[2 * r + 1] = sum;
             } else if (p.a.lse) {
               p.a.lse[int64_t(cur.b) * p.a.H + h0 + r] = sum == 0.f ? -INFINITY : (base[nh][c] + log2f(sum)) * kLn2;
             }
@@ -577,6 +613,41 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     cursor_next<kTile>(p, cur);
   }
   if (!ok && p.err) atomicExch(p.err, kErrBulkTimeout);
+  if (joins) {
+    // ---- the parts of the cluster's CTAs, in their order; each CTA adds up some of the heads, a channel per thread ----
+    const int blk = start.head % p.blocks, item_h0 = start.head / p.blocks * p.group + blk * kRows, item_rows = min(kRows, p.group - blk * kRows);
+    const unsigned ml_u = ring_u + unsigned(kRows * DP * sizeof(float));
+    if (n_my <= 0 && tid < kRows) {
+      float* part_ml = reinterpret_cast<float*>(ring) + kRows * DP;
+      part_ml[2 * tid] = -INFINITY, part_ml[2 * tid + 1] = 0.f;
+    }
+    cluster_meet();
+    for (int r = int(blockIdx.x) % p.cluster; r < item_rows; r += p.cluster) {
+      float m[8], l[8], mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        m[c] = -INFINITY, l[c] = 0.f;
+        if (c < p.cluster) ld_cluster2(ml_u + unsigned(r * 8), unsigned(c), m[c], l[c]);
+        mx = fmaxf(mx, m[c]);
+      }
+      const float top = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f, out = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        const float f = ex2_approx(m[c] - top);
+        if (c < p.cluster && l[c] != 0.f && tid < D) {  // a part without a tile has no output
+          sum = fmaf(l[c], f, sum);
+          out = fmaf(ld_cluster(ring_u + unsigned((r * DP + tid) * 4), unsigned(c)), f, out);
+        }
+      }
+      if (tid < D) {
+        const int64_t at = int64_t(start.b) * p.a.H + item_h0 + r;
+        p.a.out[at * D + tid] = mxk_bf16(pack_bf16(sum > 0.f || sum != sum ? out / sum : 0.f, 0.f) & 0xffffu);
+        if (tid == 0 && p.a.lse) p.a.lse[at] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+      }
+    }
+    cluster_meet();  // nobody goes while its shared memory is read
+  }
 }
 
 // Adds up, for each (sequence, head) that several runs share, the parts in the order of the runs: one CTA per work item and
@@ -663,18 +734,39 @@ template <bool E4M3, int DP, int NH>
 int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   constexpr int kRows = 8 * NH, kTile = DecodeCfg<E4M3, DP>::kTile;
   p.ctas = decode_ctas<E4M3, DP, NH>();
+  // tiles that a work item can have
+  int64_t tokens = int64_t(p.c.max_pages) * p.c.page_size;
+  if (p.a.left >= 0 && p.a.left < tokens && p.a.sinks < tokens - p.a.left) tokens = p.a.left + 1 + p.a.sinks;
+  const int64_t item_tiles = ceil_div(tokens, kTile), items = int64_t(p.c.n_seqs) * p.heads;
   // no more runs than there can be tiles
-  const int64_t most = int64_t(p.c.n_seqs) * p.heads * ceil_div(int64_t(p.c.max_pages) * p.c.page_size, kTile);
-  if (p.ctas > most) p.ctas = int(most < 1 ? 1 : most);
+  const int resident = p.ctas;
+  if (p.ctas > items * item_tiles) p.ctas = int(items * item_tiles < 1 ? 1 : items * item_tiles);
   const int64_t need = int64_t(2) * p.ctas * kRows * (DP + 2) * int64_t(sizeof(float));
   if (p.a.workspace_bytes < need)
     return fail(MXK_ERR_INVALID_ARG, "%s: workspace of %lld bytes, mxk_attn_decode_workspace_bytes() asks for up to %lld", name, (long long)p.a.workspace_bytes,
                 (long long)need);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
+  // The short form: as many CTAs per work item (1, 2, 4, 8) as the GPU holds at once and the item has tiles.
+  int c = 1;
+  while (c < 8 && items * c * 2 <= resident && c < item_tiles) c *= 2;
+  if (ceil_div(item_tiles, c) <= kShort) {
+    p.cluster = c;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP>::kSmem, cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(c), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, decode_kernel<E4M3, DP, NH>, p);  // errors surface through cudaGetLastError() in after_launch()
+    return after_launch(name);
+  }
+  p.cluster = 0;
   launch_pdl(decode_kernel<E4M3, DP, NH>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
   if (int rc = after_launch(name)) return rc;
-  launch_pdl(join_kernel<DP, kTile, NH>, dim3(unsigned(p.c.n_seqs * p.heads), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
+  launch_pdl(join_kernel<DP, kTile, NH>, dim3(unsigned(items), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
   return after_launch(name);
 }
 
