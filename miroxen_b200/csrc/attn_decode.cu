@@ -15,8 +15,11 @@
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
 // sum and unnormalised output in its slots of the workspace (one for the segment its run starts in, one for the segment
 // it ends in) and join_kernel, launched behind it, adds them up in order.  Where the whole call is short, that second launch is
-// most of it: if all work items cut into at most 8 fit the GPU at once with at most kShort tiles for each CTA, the CTAs of an item are
-// a cluster and add up through each other's shared memory.  Results do not depend on timing.
+// most of it: if up to 8 CTAs for each (sequence, head), as many as the GPU holds, leave at most kShort tiles for each, they are a
+// cluster and add up through each other's shared memory (1 sequence of 500 tokens, 8 key heads of 128: 5.5 against 8.0 us;
+// 32 of 300: 8.9 against 12.8).  And where there are more (sequence, head)s than CTAs by half, each of kMedium tiles at
+// most, a CTA takes one as a whole: the heads of the same tokens, which lie side by side in a page, are then read at the
+// same time (200 sequences of 2000 tokens: 252 against 278 us).  Results do not depend on timing.
 //
 // Within a CTA two warps bring the tiles of K and V into a ring of shared-memory stages (16-byte cp.async, rows found
 // through the page table one tile ahead, completion counted on mbarriers) and four warps do the arithmetic.  For the scores
@@ -40,7 +43,7 @@ namespace {
 constexpr int kWarps = 4;       // that compute
 constexpr int kCopyWarps = 2;   // that copy, 32 tokens of a tile each
 constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32 * kCopyWarps;
-constexpr int kShort = 8;       // tiles of a CTA up to which a call takes the form without a second launch
+constexpr int kShort = 8, kMedium = 32;  // tiles of a CTA up to which a call takes the forms without a second launch
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -747,10 +750,12 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
                 (long long)need);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
-  // The short form: as many CTAs per work item (1, 2, 4, 8) as the GPU holds at once and the item has tiles.
+  // The short form: as many CTAs per work item (1, 2, 4, 8) as the GPU holds at once and the item has tiles.  (Whole items
+  // against runs: 64 sequences of 2000 bf16 tokens, 512 items on 296 CTAs, 85 against 96 us; 40 of 1024, 320 items, 40 against 38
+  // us; 200 of 1024 e4m3 tokens, 1600 items on 740 CTAs, 65 against 74 us; 64 of 2000, 512 items, 49 against 45 us.)
   int c = 1;
   while (c < 8 && items * c * 2 <= resident && c < item_tiles) c *= 2;
-  if (ceil_div(item_tiles, c) <= kShort) {
+  if (ceil_div(item_tiles, c) <= (2 * items >= 3 * int64_t(resident) ? kMedium : kShort) && items * c < (int64_t(1) << 31)) {
     p.cluster = c;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP>::kSmem, cfg.stream = s;
