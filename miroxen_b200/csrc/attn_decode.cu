@@ -9,7 +9,7 @@
 // V^T P^T.  The tensor pipe is far from busy at this ratio, and the operands come from shared memory tiles that change with
 // every use, which is what the warp-level instruction takes without a detour.
 //
-// Split: a tile is 64 or 128 tokens of one (sequence, key head, block of query heads).  All tiles of the call in order
+// Split: a tile is 64 tokens of one (sequence, key head, block of query heads).  All tiles of the call in order
 // (sequence, head, token) are cut into equal runs, one per resident CTA, whatever the lengths are - a CTA's run may
 // end inside a sequence's tokens and cover several short sequences.  Each CTA finds the run's start itself by summing the
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
@@ -29,6 +29,10 @@
 // it, so the result is the same): one barrier per tile, which also carries that vote.
 // Scores, maxima, sums and output are fp32; probabilities are rounded to bf16 (f16 for an e4m3 cache) for the product, as
 // the tensor instruction needs the type of V.
+//
+// Measured (floor at 6560 GB/s in brackets): 64 sequences of 4100 to 16384 bf16 tokens, 32 heads on 8 of 128, pages of 16:
+// 407 us (382); 8 sequences with 32833 e4m3 tokens in view, 40 heads on 8: 100 us (82); 48 of 2250 to 9000 e4m3 tokens, 28 heads
+// on 4 of 64: 43 us (22 - rows of 64 bytes that do not lie next to each other: half of each line that is asked for).
 #include <cuda_fp16.h>
 
 #include <type_traits>

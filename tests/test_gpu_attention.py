@@ -612,3 +612,46 @@ def test_a_prompt_and_then_single_tokens(mx, kind):
             else:  # e4m3: each k and v off by 2^-4 of itself at most (and 2^-10 steps), a score by 2^-4 of its products
                 size = D ** -0.5 * (q1[b].float().abs().view(H, D).amax(1) * torch.stack(keys[b]).float().abs().sum(-1).amax())
                 assert bool(((o1[b].double() - ref[0][0]).norm(dim=1) <= ref[0][0].norm(dim=1) + 4).all()) and bool(size.isfinite().all())
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_decode_wide_tables_and_short_sequences(mx, kind):
+    """Tables with room for far more tokens than there are (the call cannot know), and the same lengths in tables that just
+    hold them: other splits of the work, both right."""
+    g = gen(25)
+    lens = [300, 0, 1, 64, 65, 700]
+    cache = make_cache(mx, g, kind, 6, 700, 16, 2, 128)
+    wide = torch.full((6, 4000), -1, device="cuda", dtype=torch.int32)
+    wide[:, :cache.page_table.shape[1]] = cache.page_table
+    for table in (cache.page_table, wide):
+        c = mx.KvCache(cache.k, cache.v, table, cache.k_scale, cache.v_scale)
+        check_decode(mx, 26, kind, lens, 10, 2, 128, 16, cache=c)
+        check_decode(mx, 27, kind, lens, 40, 2, 128, 16, left=90, sinks=3, cache=c)
+
+
+def test_two_streams_at_once(mx):
+    """The three calls on two streams at the same time, a workspace each: what they give one after the other."""
+    g = gen(60)
+    jobs = []
+    for i in range(2):
+        cache = make_cache(mx, g, BF16, 4, 3000, 16, 2, 128)
+        q, qkv = rand(g, 4, 8, 128), rand(g, 2000, 12 * 128)
+        jobs.append((cache, q, torch.tensor([3000, 17, 1500 + i, 900], device="cuda", dtype=torch.int32), mx.attn_decode_workspace(cache, 8), qkv))
+
+    def run(job, stream):
+        cache, q, lens, ws, qkv = job
+        out, big = torch.empty(4, 8, 128, device="cuda", dtype=torch.bfloat16), torch.empty(2000, 8, 128, device="cuda", dtype=torch.bfloat16)
+        stream.wait_stream(torch.cuda.current_stream())
+        for _ in range(5):
+            mx.attn_window(qkv, qkv[:, 1024:], qkv[:, 1280:], 2000, 2000, 8, 2, 128, 0.088, big, left=300, right=0, sinks=4, q_stride=1536, k_stride=1536,
+                           v_stride=1536, stream=stream)
+            mx.attn_decode_paged(q, cache, lens, 8, 0.088, out, workspace=ws, stream=stream)
+        return out, big
+
+    one = [run(j, torch.cuda.default_stream()) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    two = [run(j, s) for j, s in zip(jobs, streams)]
+    torch.cuda.synchronize()
+    for a, b in zip(one, two):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
