@@ -31,7 +31,7 @@
 // Measured (D = 128): 2 x 4352 rows x 24 heads, everything visible, 360 us = 1290 TFLOP/s from a cold start, 429 us = 1085
 // TFLOP/s in a run of seconds, where the power limit holds the clock near 1530 MHz (a library product: 1651 and 1393);
 // 33272 rows x 5 heads with a window of 6240 each way and 1560 first keys 800 us; nine packed causal prompts of 14 to 3414 rows,
-// 32 heads on 8, window 1024: 114 us; one prompt of 77 rows: 7.3 us.  What bounds it: the tensor pipe, busy 69 % of the time
+// 32 heads on 8, window 1024: 113 us; one prompt of 77 rows: 6.9 us.  What bounds it: the tensor pipe, busy 69 % of the time
 // (the scores' operands both come from shared memory, 98 clocks instead of 64 per product), and the last round of tiles.
 #include <cuda.h>
 
@@ -739,23 +739,24 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       const uint64_t f2 = pair(f, f);
       uint64_t odd2 = 0;  // becomes NaN with an output that is not finite
       mxk_bf16* dst = a.out + (row0 + (lane >> 3)) * a.out_stride + int64_t(t.head) * a.D + 8 * (lane & 7);
-#pragma unroll 1
-      for (int c = 0; c < DP / 64; c++) {
-        unsigned o[2][32];
-        if (done == 0) {
+      unsigned o[DP / 32][32];
+      if (done == 0) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) o[0][i] = o[1][i] = 0u;
-        } else {
-          tmem_ld32(to + 64 * c, o[0]);
-          tmem_ld32(to + 64 * c + 32, o[1]);
-          tmem_wait_ld(o[0]);
-          tmem_touch(o[1]);
-          if (c == DP / 64 - 1) {  // the next tile's output may come
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive1(smem_u32(&sm.o_empty[h]));
-          }
-        }
+        for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[c][i] = 0u;
+      } else {
+#pragma unroll
+        for (int c = 0; c < DP / 32; c++) tmem_ld32(to + 32 * c, o[c]);
+        tmem_wait_ld(o[0]);
+#pragma unroll
+        for (int c = 1; c < DP / 32; c++) tmem_touch(o[c]);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(smem_u32(&sm.o_empty[h]));  // the next tile's output may come
+      }
+#pragma unroll
+      for (int c = 0; c < DP / 64; c++) {
         // A row per lane from tensor memory, 128 bytes of four rows per store to memory: through shared memory, the 16-byte
         // chunks of a row exchanged by the row's number.
 #pragma unroll
@@ -764,7 +765,8 @@ __global__ void __launch_bounds__(kThreadsW, 1)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int k = 8 * (i & 3) + 2 * e;
-            const uint64_t x = fma2(pair(__uint_as_float(o[i >> 2][k]), __uint_as_float(o[i >> 2][k + 1])), f2, 0);  // 0 * 0 in a row that sees nothing
+            const unsigned(&r)[32] = o[2 * c + (i >> 2)];
+            const uint64_t x = fma2(pair(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), f2, 0);  // 0 * 0 in a row that sees nothing
             odd2 = fma2(x, 0, odd2);
             float lo, hi;
             split(x, lo, hi);
