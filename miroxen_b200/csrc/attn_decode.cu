@@ -49,6 +49,10 @@ constexpr int kCopyWarps = 2;   // that copy, 32 tokens of a tile each
 constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32 * kCopyWarps;
 constexpr int kShort = 8, kMedium = 32;  // tiles of a CTA up to which a call takes the forms without a second launch
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
+// Probabilities in f16 (of an e4m3 cache) are taken relative to a maximum 2^7 lower than the scores': they reach 2^15 then, which
+// f16 holds, and what it rounds them to at the small end is 2^-32 of the largest instead of 2^-25 (a million tokens that are
+// each that small are 3 % of the sum).
+constexpr float kLift = 7.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DecodeLaunch {
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   // this warp's state.  Column c of a product is query head 8 nh + c; a lane holds columns 2 c2 and 2 c2 + 1 of rows r0 and
   // r0 + 8 (tokens of the scores, channels of the output), as a right operand column r0.
   float o[kMT][NH][4];
-  float base[NH][2], l[NH][2], scale[NH][2];  // maximum in use (in units of log2), this thread's part of the sum, of the columns
+  float base[NH][2], l[NH][2], scale[NH][2];  // maximum in use (in units of log2, less kLift), this thread's part of the sum, of the columns
   unsigned qf[NH][kKSteps][2];
   const int r0 = lane >> 2, c2 = lane & 3;
   const Cursor start = cur;
@@ -474,6 +478,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
         mx[nh][c] = fmaxf(s[0][nh][c], s[0][nh][2 + c]);
 #pragma unroll
         for (int t = 1; t < kTT; t++) mx[nh][c] = fmaxf(mx[nh][c], fmaxf(s[t][nh][c], s[t][nh][2 + c]));
+        if (E4M3) mx[nh][c] -= kLift;
         grows |= mx[nh][c] > base[nh][c] + kSlack;
       }
     }

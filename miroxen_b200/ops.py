@@ -38,7 +38,7 @@ __all__ = [
 
 
 def _p(t) -> Optional[int]:
-    return t if t is None or t.__class__ is int else t.data_ptr()
+    return t if t is None or isinstance(t, int) else t.data_ptr()
 
 
 # The current stream's handle without a Stream object around it (0.3 instead of 3.2 us per call, which is most of what a

@@ -1,8 +1,8 @@
 """Plain 64-bit forms of the attention operators and how far the kernels may be off them.
 
 Bounds.  With w_j the softmax weights and A = sum_j w_j |v_j|: rounding the output to bf16 is off by at most 2^-8 of it;
-rounding each weight before the product with V (bf16: 2^-8, f16: 2^-11 of the weight, and 2^-25 of the largest weight
-where it is subnormal in f16) moves the output by at most that share of A; a score off by d changes every weight by at
+rounding each weight before the product with V (bf16: 2^-8, f16: 2^-11 of the weight, and 2^-32 of the largest weight
+where it is subnormal in f16: half a step, 2^-25, of weights the largest of which is taken as 2^7 or more) moves the output by at most that share of A; a score off by d changes every weight by at
 most a factor exp(2 d).  Scores are fp32 sums of D products: each of the D additions and the scaling rounds by 2^-24 of
 at most S = max scale sum |q_d k_d|, and 2^x of the hardware is good to 2^-22, the sums of the weights to 2^-20.
 """
@@ -78,7 +78,7 @@ def decode_reference(q, cache, lens, H, scale, left, sinks):
             g = h // (H // Hkv)
             ks, vs = (1.0 if s is None else float(s[g]) for s in (cache.k_scale, cache.v_scale))
             o, l, bo, bl = attention_rows(q[b, h][None], k[:, g] * ks, v[:, g] * vs, scale, see, 2.0 ** -11 if e4m3 else 2.0 ** -8,
-                                          2.0 ** -25 if e4m3 else 0.0)
+                                          2.0 ** -32 if e4m3 else 0.0)
             outs[0][b, h], outs[1][b, h], lses[0][b, h], lses[1][b, h] = o[0], bo[0], l[0], bl[0]
     return outs[0], lses[0], outs[1], lses[1]
 

@@ -364,6 +364,31 @@ def test_decode_offsets_past_32_bits(mx):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_decode_many_small_weights(mx, kind):
+    """A million tokens of weight 2^-25.1 behind one of weight 1, as many work items as fill the GPU with such runs: what the
+    small ones add up to must not be lost in the type that the product with V takes them in."""
+    seqs, Hkv, D, page, pages = 64, 8, 64, 64, 16384
+    L, bits = page * pages, 25.1
+    k, v = torch.full((2, page, Hkv, D), -1.0, device="cuda"), torch.full((2, page, Hkv, D), 448.0, device="cuda")
+    k[0, 0], v[0, 0] = 0.0, 2.0 ** -4
+    dtype = torch.bfloat16 if kind == BF16 else torch.float8_e4m3fn
+    table = torch.ones(seqs, pages, dtype=torch.int32, device="cuda")
+    table[:, 0] = 0
+    cache = mx.KvCache(k.to(dtype), v.to(dtype), table)
+    q = torch.ones(seqs, Hkv, D, dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(seqs, Hkv, device="cuda")
+    lens = torch.full((seqs,), L, dtype=torch.int32, device="cuda")
+    mx.attn_decode_paged(q, cache, lens, Hkv, bits * math.log(2) / D, out, lse=lse, workspace=mx.attn_decode_workspace(cache, Hkv))
+    small = (L - 1) * 2.0 ** -bits
+    want = (2.0 ** -4 + small * 448) / (1 + small)
+    # fp32 sums over a run: one step of 2^-23 for each of its L / 16 products, of the output's largest partial sum, which is
+    # the output; a thread's sum of weights takes one step of 2^-23 for each of its L / 64 tiles
+    steps = L / 16 * 2.0 ** -23
+    assert (out.double() - want).abs().max().item() <= want * (2.0 ** -8 + 2.0 ** -8 + 2 * steps)
+    assert (lse.double() - math.log1p(small)).abs().max().item() <= L / 64 * 2.0 ** -23 + 2.0 ** -20
+
+
 def test_decode_in_a_graph_on_another_stream(mx):
     """Captured once, replayed with other lengths, queries and tables: the call reads all of them on the device."""
     g = gen(23)
