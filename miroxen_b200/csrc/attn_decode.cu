@@ -212,11 +212,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two e4m3 values (exact in f16)
-__device__ __forceinline__ unsigned e4m3x2_to_f16x2(unsigned pair) {
-  unsigned r;
-  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(pair));
-  return r;
+// Four e4m3 values as f16, which holds them exactly: bytes 0, 1 and bytes 2, 3.
+__device__ __forceinline__ void e4m3x4_to_f16(unsigned x, unsigned& lo, unsigned& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(x));
 }
 __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -452,8 +450,8 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
           ldsm4(a + unsigned(t * 16 * kPitch + ks * 16), w);
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            const unsigned k[4] = {e4m3x2_to_f16x2(w[2 * x] & 0xffffu), e4m3x2_to_f16x2(w[2 * x + 1] & 0xffffu), e4m3x2_to_f16x2(w[2 * x] >> 16),
-                                   e4m3x2_to_f16x2(w[2 * x + 1] >> 16)};
+            unsigned k[4];
+            e4m3x4_to_f16(w[2 * x], k[0], k[2]), e4m3x4_to_f16(w[2 * x + 1], k[1], k[3]);
 #pragma unroll
             for (int nh = 0; nh < NH; nh++) mma16816<true>(s[t][nh], k, qf[nh][ks + x][0], qf[nh][ks + x][1]);
           }
@@ -558,9 +556,8 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
           ldsm4_t(v_u + unsigned((k2 * 32 + lane) * kPitch + (warp * kMT + m) * 16), v);
 #pragma unroll
           for (int ks = 0; ks < 2; ks++) {
-            const unsigned lo = v[2 * ks], hi = v[2 * ks + 1];
-            const unsigned a[4] = {e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(lo, 0, 0x4431)),
-                                   e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4420)), e4m3x2_to_f16x2(__byte_perm(hi, 0, 0x4431))};
+            unsigned a[4];
+            e4m3x4_to_f16(__byte_perm(v[2 * ks], 0, 0x3120), a[0], a[1]), e4m3x4_to_f16(__byte_perm(v[2 * ks + 1], 0, 0x3120), a[2], a[3]);
 #pragma unroll
             for (int nh = 0; nh < NH; nh++) mma16816<true>(o[m][nh], a, pb[nh][2 * ks], pb[nh][2 * ks + 1]);
           }
