@@ -9,7 +9,7 @@
 // V^T P^T.  The tensor pipe is far from busy at this ratio, and the operands come from shared memory tiles that change with
 // every use, which is what the warp-level instruction takes without a detour.
 //
-// Split: a tile is 64 tokens of one (sequence, key head, block of query heads).  All tiles of the call in order
+// Split: a tile is 64 or 128 tokens of one (sequence, key head, block of query heads).  All tiles of the call in order
 // (sequence, head, token) are cut into equal runs, one per resident CTA, whatever the lengths are - a CTA's run may
 // end inside a sequence's tokens and cover several short sequences.  Each CTA finds the run's start itself by summing the
 // lengths.  A run that covers a (sequence, head) alone writes its output; otherwise the CTA leaves its running maximum,
@@ -222,27 +222,32 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
 }
 
 // A stage holds a tile of K and one of V, a row per token, rows 16 bytes longer than their DP elements: the eight rows that
-// an ldmatrix phase reads then start four banks apart.  A tile has 64 tokens, 16 for each computing warp: tiles of 128 tokens
-// cost the e4m3 kernels a CTA per SM and were slower or equal.  Stages: as many as leave two (bf16, D > 64) to four CTAs per
-// SM, whose number counts for more than the depth of a ring: 8 sequences of 32832 e4m3 tokens in view take 99.7 us with two
-// stages, 102.5 with three and 102.5 with four; 64 sequences of bf16, D = 128, 421 us with three stages, 455 with two,
-// 804 with four (one CTA per SM).
-template <bool E4M3, int DP>
+// an ldmatrix phase reads then start four banks apart.  A tile has 16 tokens for each computing warp; 32 (LONG) where rows are
+// short, D <= 64, and the call is cut into runs.  Stages: as many as leave
+//   two CTAs per SM to bf16 rows of D > 64 (64 long sequences: 421 us with three stages, 455 with two and three CTAs, 804 with four
+//   and one) and to LONG tiles (48 sequences of up to 9000 tokens, 4 heads of 64: e4m3 38 us against 42 with tiles of 64 and four
+//   CTAs, 46 with one CTA; bf16 56 against 75 with three CTAs and 58 with tiles of 64 and two) - fewer rows of the memory are then
+//   open at a time;
+//   as many CTAs as there are registers for to the other e4m3 rows (8 sequences with 32832 tokens in view, D = 128: 95 us with two
+//   stages, 102.5 with three or four, 112 with LONG tiles), which take more arithmetic per byte, and to short calls, where a CTA has
+//   few tiles (300 sequences of 600 tokens, 4 heads of 64: e4m3 22 us against 28, bf16 30 against 34 with LONG tiles).
+template <bool E4M3, int DP, bool LONG>
 struct DecodeCfg {
-  static constexpr int kTokW = 16;  // tokens per warp
+  static_assert(!LONG || DP == 64, "LONG tiles belong to short rows");
+  static constexpr int kTokW = LONG ? 32 : 16;  // tokens per warp
   static constexpr int kTile = kTokW * kWarps;
-  static_assert(kTile == 32 * kCopyWarps, "a copying warp looks up a token per lane");
+  static constexpr int kPerLane = kTile / (32 * kCopyWarps);  // tokens that a lane of a copying warp looks up
   static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2), kPitch = kRowBytes + 16;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kTileBytes = kTile * kPitch;
-  static constexpr int kStages = DP == 64 ? 4 : E4M3 ? 2 : 3;
+  static constexpr int kStages = LONG ? (E4M3 ? 5 : 2) : DP == 64 ? 4 : E4M3 ? 2 : 3;
   static constexpr int kSmem = kStages * 2 * kTileBytes;
 };
 
 // NH: blocks of 8 query heads.
-template <bool E4M3, int DP, int NH>
+template <bool E4M3, int DP, int NH, bool LONG>
 __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant__ DecodeLaunch p) {
-  using Cfg = DecodeCfg<E4M3, DP>;
+  using Cfg = DecodeCfg<E4M3, DP, LONG>;
   using elem = typename KvElem<E4M3>::type;
   constexpr int kSt = Cfg::kStages, kTile = Cfg::kTile, kTokW = Cfg::kTokW, kPitch = Cfg::kPitch, kRows = 8 * NH;
   constexpr int kKSteps = DP / 16, kMT = DP / kWarps / 16, kTT = kTokW / 16;  // 16-channel steps, 16-channel tiles, 16-token tiles of a warp
@@ -305,48 +310,61 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     const bool copies = ch * 16 < D * int(sizeof(elem));
     const unsigned char* kb = static_cast<const unsigned char*>(p.c.k) + ch * 16;
     const int64_t to_v = static_cast<const unsigned char*>(p.c.v) - static_cast<const unsigned char*>(p.c.k);
-    // Page and slot of token 32 part + lane of the tile that is copied next (slot -1: no token), asked for before the tile in
-    // front of it is copied and not looked at until then, so that the page table's latency passes meanwhile.
-    int page, slot;
+    // Page and slot of tokens 32 (kPL part + x) + lane of the tile that is copied next (slot -1: no token), asked for before the
+    // tile in front of it is copied and not looked at until then, so that the page table's latency passes meanwhile.
+    constexpr int kPL = Cfg::kPerLane;
+    int page[kPL], slot[kPL];
     int64_t head_off;
     auto look_up = [&]() {
       head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
-      const int i = cur.tile * kTile + part * 32 + lane;
-      page = 0, slot = -1;
-      if (i < cur.v.len) {  // inside the table: the length is held to it
-        const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
-        // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
-        int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
-        if (r >= p.c.page_size) n++, r -= p.c.page_size;
-        slot = r;
-        page = p.c.page_table[int64_t(cur.b) * p.c.table_stride + n];
+#pragma unroll
+      for (int x = 0; x < kPL; x++) {
+        const int i = cur.tile * kTile + (part * kPL + x) * 32 + lane;
+        page[x] = 0, slot[x] = -1;
+        if (i < cur.v.len) {  // inside the table: the length is held to it
+          const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
+          // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
+          int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
+          if (r >= p.c.page_size) n++, r -= p.c.page_size;
+          slot[x] = r;
+          page[x] = p.c.page_table[int64_t(cur.b) * p.c.table_stride + n];
+        }
       }
       cursor_next<kTile>(p, cur);
     };
     look_up();
     int st = 0;
     for (int i = 0; i < n_my; i++) {
-      int64_t off = -1;  // byte offset, -1: not there
-      if (slot >= 0) {
-        if (page >= 0 && page < p.c.num_pages) off = (int64_t(page) * p.c.page_stride + int64_t(slot) * p.c.token_stride + head_off) * int(sizeof(elem));
-        else if (p.err) atomicExch(p.err, kErrBadIndex);
+      int64_t off[kPL];  // byte offsets, -1: not there
+#pragma unroll
+      for (int x = 0; x < kPL; x++) {
+        off[x] = -1;
+        if (slot[x] >= 0) {
+          if (page[x] >= 0 && page[x] < p.c.num_pages)
+            off[x] = (int64_t(page[x]) * p.c.page_stride + int64_t(slot[x]) * p.c.token_stride + head_off) * int(sizeof(elem));
+          else if (p.err)
+            atomicExch(p.err, kErrBadIndex);
+        }
       }
       if (i + 1 < n_my) look_up();
       if (i >= kSt) {
         ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u));
         if (!ok) break;
       }
-      const unsigned dk = ring_u + unsigned(st) * 2 * Cfg::kTileBytes + unsigned((part * 32 + sub) * kPitch + ch * 16);
-      const unsigned word = __ballot_sync(0xffffffffu, off >= 0);
-      if (lane == 0) there[st][part] = word;
 #pragma unroll
-      for (int r = 0; r < 32 / kPerInstr; r++) {
-        const int64_t o = __shfl_sync(0xffffffffu, off, r * kPerInstr + sub);
-        if (copies) {  // a token that is not there reads as zeros: its value must not carry anything into 0 * v
-          const unsigned n = o >= 0 ? 16u : 0u;
-          const unsigned char* x = kb + (o >= 0 ? o : 0);
-          cp_async16(dk + unsigned(r * kPerInstr * kPitch), x, n);
-          cp_async16(dk + unsigned(Cfg::kTileBytes + r * kPerInstr * kPitch), x + to_v, n);
+      for (int x = 0; x < kPL; x++) {
+        const unsigned dk = ring_u + unsigned(st) * 2 * Cfg::kTileBytes + unsigned(((part * kPL + x) * 32 + sub) * kPitch + ch * 16);
+        const unsigned word = __ballot_sync(0xffffffffu, off[x] >= 0);
+        if (lane == 0) there[st][part * kPL + x] = word;
+#pragma unroll
+        for (int r = 0; r < 32 / kPerInstr; r++) {
+          const int64_t o = __shfl_sync(0xffffffffu, off[x], r * kPerInstr + sub);
+          if (copies) {  // a token that is not there reads as zeros: its value must not carry anything into 0 * v
+            const unsigned n = o >= 0 ? 16u : 0u;
+            const unsigned char* from = kb + (o >= 0 ? o : 0);
+            cp_async16(dk + unsigned(r * kPerInstr * kPitch), from, n);
+            cp_async16(dk + unsigned(Cfg::kTileBytes + r * kPerInstr * kPitch), from + to_v, n);
+          }
         }
       }
       cp_async_arrive(smem_u32(&full[st]));
@@ -459,7 +477,8 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     }
     // the warp's bits of the tile's tokens
     const unsigned word = there[st][warp * kTokW / 32] >> (warp * kTokW % 32);
-    const bool all_there = (word & 0xffffu) == 0xffffu;
+    constexpr unsigned kAll = kTokW == 32 ? 0xffffffffu : 0xffffu;
+    const bool all_there = (word & kAll) == kAll;
     float mx[NH][2];
     bool grows = false;
 #pragma unroll
@@ -732,23 +751,24 @@ __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant_
   if (tid == 0 && p.a.lse) p.a.lse[int64_t(b) * p.a.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-template <bool E4M3, int DP, int NH>
+// CTAs that the GPU holds at once.
+template <bool E4M3, int DP, int NH, bool LONG>
 int decode_ctas() {
-  auto k = decode_kernel<E4M3, DP, NH>;
-  allow_smem(k, DecodeCfg<E4M3, DP>::kSmem);  // a failure surfaces at the launch
-  return sm_count() * resident_ctas(k, kThreadsD, DecodeCfg<E4M3, DP>::kSmem);
+  auto k = decode_kernel<E4M3, DP, NH, LONG>;
+  allow_smem(k, DecodeCfg<E4M3, DP, LONG>::kSmem);  // a failure surfaces at the launch
+  return sm_count() * resident_ctas(k, kThreadsD, DecodeCfg<E4M3, DP, LONG>::kSmem);
 }
 
 template <bool E4M3, int DP, int NH>
 int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
-  constexpr int kRows = 8 * NH, kTile = DecodeCfg<E4M3, DP>::kTile;
-  p.ctas = decode_ctas<E4M3, DP, NH>();
-  // tiles that a work item can have
+  constexpr bool kLong = DP == 64;  // of the form with runs
+  constexpr int kRows = 8 * NH, kTile = DecodeCfg<E4M3, DP, kLong>::kTile, kShortTile = DecodeCfg<E4M3, DP, false>::kTile;
+  p.ctas = decode_ctas<E4M3, DP, NH, kLong>();
+  // tokens and tiles that a work item can have
   int64_t tokens = int64_t(p.c.max_pages) * p.c.page_size;
   if (p.a.left >= 0 && p.a.left < tokens && p.a.sinks < tokens - p.a.left) tokens = p.a.left + 1 + p.a.sinks;
   const int64_t item_tiles = ceil_div(tokens, kTile), items = int64_t(p.c.n_seqs) * p.heads;
   // no more runs than there can be tiles
-  const int resident = p.ctas;
   if (p.ctas > items * item_tiles) p.ctas = int(items * item_tiles < 1 ? 1 : items * item_tiles);
   const int64_t need = int64_t(2) * p.ctas * kRows * (DP + 2) * int64_t(sizeof(float));
   if (p.a.workspace_bytes < need)
@@ -759,23 +779,24 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   // The short form: as many CTAs per work item (1, 2, 4, 8) as the GPU holds at once and the item has tiles.  (Whole items
   // against runs: 64 sequences of 2000 bf16 tokens, 512 items on 296 CTAs, 85 against 96 us; 40 of 1024, 320 items, 40 against 38
   // us; 200 of 1024 e4m3 tokens, 1600 items on 740 CTAs, 65 against 74 us; 64 of 2000, 512 items, 49 against 45 us.)
+  const int64_t resident = decode_ctas<E4M3, DP, NH, false>(), short_tiles = ceil_div(tokens, kShortTile);
   int c = 1;
-  while (c < 8 && items * c * 2 <= resident && c < item_tiles) c *= 2;
-  if (ceil_div(item_tiles, c) <= (2 * items >= 3 * int64_t(resident) ? kMedium : kShort) && items * c < (int64_t(1) << 31)) {
+  while (c < 8 && items * c * 2 <= resident && c < short_tiles) c *= 2;
+  if (ceil_div(short_tiles, c) <= (2 * items >= 3 * resident ? kMedium : kShort) && items * c < (int64_t(1) << 31)) {
     p.cluster = c;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP>::kSmem, cfg.stream = s;
+    cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP, false>::kSmem, cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = unsigned(c), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at, cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, decode_kernel<E4M3, DP, NH>, p);  // errors surface through cudaGetLastError() in after_launch()
+    cudaLaunchKernelEx(&cfg, decode_kernel<E4M3, DP, NH, false>, p);  // errors surface through cudaGetLastError() in after_launch()
     return after_launch(name);
   }
   p.cluster = 0;
-  launch_pdl(decode_kernel<E4M3, DP, NH>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP>::kSmem, s, p);
+  launch_pdl(decode_kernel<E4M3, DP, NH, kLong>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP, kLong>::kSmem, s, p);
   if (int rc = after_launch(name)) return rc;
   launch_pdl(join_kernel<DP, kTile, NH>, dim3(unsigned(items), unsigned(p.group < kRows ? p.group : kRows)), dim3(kConsumers), 0, s, p);
   return after_launch(name);
@@ -808,7 +829,7 @@ int64_t mxk_attn_decode_workspace_bytes(const MxkKvCache* cache, int H) {
   if (int rc = check_cache(name, cache)) return rc;
   if (int rc = check_heads(name, cache, H)) return rc;
   const int64_t bytes = pick_decode(cache, H / cache->Hkv, [](auto e, auto dp, auto nh) {
-    return int64_t(2) * decode_ctas<e.value != 0, dp.value, nh.value>() * (8 * nh.value) * (dp.value + 2) * int64_t(sizeof(float));
+    return int64_t(2) * decode_ctas<e.value != 0, dp.value, nh.value, dp.value == 64>() * (8 * nh.value) * (dp.value + 2) * int64_t(sizeof(float));
   });
   cudaGetLastError();  // without a GPU the size is that of the usual one
   return bytes;
