@@ -17,7 +17,7 @@
 // it ends in) and join_kernel, launched behind it, adds them up in order.  Where the whole call is short, that second launch is
 // most of it: if up to 8 CTAs for each (sequence, head), as many as the GPU holds, leave at most kShort tiles for each, they are a
 // cluster and add up through each other's shared memory (1 sequence of 500 tokens, 8 key heads of 128: 5.5 against 8.0 us;
-// 32 of 300: 8.9 against 12.8).  And where there are more (sequence, head)s than CTAs by half, each of kMedium tiles at
+// 32 of 300: 8.6 against 12.8).  And where there are more (sequence, head)s than CTAs by half, each of kMedium tiles at
 // most, a CTA takes one as a whole: the heads of the same tokens, which lie side by side in a page, are then read at the
 // same time (200 sequences of 2000 tokens: 252 against 278 us).  Results do not depend on timing.
 //
@@ -31,8 +31,9 @@
 // the tensor instruction needs the type of V.
 //
 // Measured (floor at 6560 GB/s in brackets): 64 sequences of 4100 to 16384 bf16 tokens, 32 heads on 8 of 128, pages of 16:
-// 407 us (382); 8 sequences with 32833 e4m3 tokens in view, 40 heads on 8: 100 us (82); 48 of 2250 to 9000 e4m3 tokens, 28 heads
-// on 4 of 64: 43 us (22 - rows of 64 bytes that do not lie next to each other: half of each line that is asked for).
+// 407 us (382); 8 sequences with 32833 e4m3 tokens in view, 40 heads on 8: 96 us (82); 48 of 2250 to 9000 e4m3 tokens, 28 heads
+// on 4 of 64: 38 us (22 - rows of 64 bytes take as many instructions per token as longer ones: issue slots 59 % used; with the
+// heads outermost in a page the same).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -48,6 +49,7 @@ constexpr int kWarps = 4;       // that compute
 constexpr int kCopyWarps = 2;   // that copy, 32 tokens of a tile each
 constexpr int kConsumers = 32 * kWarps, kThreadsD = kConsumers + 32 * kCopyWarps;
 constexpr int kShort = 8, kMedium = 32;  // tiles of a CTA up to which a call takes the forms without a second launch
+constexpr int kSingle = 4;               // tiles of a work item up to which it is one CTA's
 constexpr float kSlack = 8.f;   // log2 of how far a score may lie above the maximum in use
 // Probabilities in f16 (of an e4m3 cache) are taken relative to a maximum 2^7 lower than the scores': they reach 2^15 then, which
 // f16 holds, and what it rounds them to at the small end is 2^-32 of the largest instead of 2^-25 (a million tokens that are
@@ -751,6 +753,8 @@ __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant_
   if (tid == 0 && p.a.lse) p.a.lse[int64_t(b) * p.a.H + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
+// A number as a type.
+template <int N> using Int = std::integral_constant<int, N>;
 // CTAs that the GPU holds at once.
 template <bool E4M3, int DP, int NH, bool LONG>
 int decode_ctas() {
@@ -776,24 +780,36 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
                 (long long)need);
   p.part_o = static_cast<float*>(p.a.workspace);
   p.part_ml = p.part_o + int64_t(2) * p.ctas * kRows * DP;
-  // The short form: as many CTAs per work item (1, 2, 4, 8) as the GPU holds at once and the item has tiles.  (Whole items
-  // against runs: 64 sequences of 2000 bf16 tokens, 512 items on 296 CTAs, 85 against 96 us; 40 of 1024, 320 items, 40 against 38
-  // us; 200 of 1024 e4m3 tokens, 1600 items on 740 CTAs, 65 against 74 us; 64 of 2000, 512 items, 49 against 45 us.)
+  // The short form: as many CTAs per work item (1, 4, 8) as the GPU holds at once and the item has tiles.  One where it has no
+  // more than kSingle tiles (16 sequences of 200 tokens, 4 heads of 64: 5.5 against 6.7 us with four, and 9.6 with two for 64 of
+  // them); two, which add up no faster than eight, only where one would be too few for this form (32 of 300: 6.7 against 8.9 us
+  // with two; but 24 of 1000, 8 heads of 128, e4m3: two 14.2 us, runs 15.6).  (Whole items against runs: 64 sequences of 2000
+  // bf16 tokens, 512 items on 296 CTAs, 85 against 96 us; 40 of 1024, 320 items, 40 against 38 us; 200 of 1024 e4m3 tokens, 1600 items
+  // on 740 CTAs, 65 against 74 us; 64 of 2000, 512 items, 49 against 45 us.)
   const int64_t resident = decode_ctas<E4M3, DP, NH, false>(), short_tiles = ceil_div(tokens, kShortTile);
   int c = 1;
-  while (c < 8 && items * c * 2 <= resident && c < short_tiles) c *= 2;
-  if (ceil_div(short_tiles, c) <= (2 * items >= 3 * resident ? kMedium : kShort) && items * c < (int64_t(1) << 31)) {
+  while (short_tiles > kSingle && c < 8 && items * c * 2 <= resident && c < short_tiles) c *= 2;
+  if (c == 2 && short_tiles <= kShort) c = 1;
+  auto one_launch = [&](auto long_tiles) {
+    constexpr bool kL = long_tiles.value != 0;
     p.cluster = c;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP, false>::kSmem, cfg.stream = s;
+    cfg.gridDim = dim3(unsigned(items * c)), cfg.blockDim = dim3(kThreadsD), cfg.dynamicSmemBytes = DecodeCfg<E4M3, DP, kL>::kSmem, cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = unsigned(c), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at, cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, decode_kernel<E4M3, DP, NH, false>, p);  // errors surface through cudaGetLastError() in after_launch()
+    cudaLaunchKernelEx(&cfg, decode_kernel<E4M3, DP, NH, kL>, p);  // errors surface through cudaGetLastError() in after_launch()
     return after_launch(name);
+  };
+  if (ceil_div(short_tiles, c) <= (2 * items >= 3 * resident ? kMedium : kShort) && items * c < (int64_t(1) << 31)) return one_launch(Int<0>());
+  // Whole items of LONG tiles where those have two CTAs per SM to fill: 200 sequences of 2000 e4m3 tokens, 4 heads of 64, 42 against
+  // 52 us by runs, of 4000 73 against 100; bf16 54 and 97 against 53 and 98.
+  if constexpr (kLong) {
+    c = 1;
+    if (item_tiles <= kMedium && 2 * items >= 3 * int64_t(decode_ctas<E4M3, DP, NH, true>()) && items < (int64_t(1) << 31)) return one_launch(Int<1>());
   }
   p.cluster = 0;
   launch_pdl(decode_kernel<E4M3, DP, NH, kLong>, dim3(unsigned(p.ctas)), dim3(kThreadsD), DecodeCfg<E4M3, DP, kLong>::kSmem, s, p);
@@ -803,7 +819,6 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
 }
 
 // The kernel for a cache and head count: f(e4m3, padded head dimension, blocks of 8 heads), as types.
-template <int N> using Int = std::integral_constant<int, N>;
 template <class F>
 auto pick_decode(const MxkKvCache* c, int group, F f) {
   const bool e = c->type == MXK_KV_E4M3, small = c->D <= 64;
