@@ -654,6 +654,35 @@ def test_decode_wide_tables_and_short_sequences(mx, kind):
         check_decode(mx, 27, kind, lens, 40, 2, 128, 16, left=90, sinks=3, cache=c)
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+@pytest.mark.parametrize("D", [48, 64])
+@pytest.mark.parametrize("group", [3, 11, 20])
+def test_decode_splits_of_short_rows(mx, kind, D, group):
+    """Rows of at most 64 channels in every split of the work: tables with room for one to many tiles and few to many sequences,
+    lengths at the edges of 64 and 128 tokens and of the pages."""
+    g = gen(28)
+    edges = [0, 1, 63, 64, 65, 127, 128, 129, 192, 255, 256, 257, 400, 479]
+    cache = make_cache(mx, g, kind, len(edges), 480, 16, 2, D)
+    for seqs, room, left, sinks in ((3, 100, -1, 0), (14, 256, -1, 0), (14, 300, 140, 5), (14, 4000, -1, 0), (14, 8000, 130, 70), (250, 4000, -1, 0), (250, 500, -1, 0)):
+        lens = [min(edges[(5 * i + 3) % len(edges)], room) for i in range(seqs)]
+        table = torch.full((seqs, -(-room // 16)), -1, device="cuda", dtype=torch.int32)
+        rows = cache.page_table[torch.arange(seqs, device="cuda") % len(edges)][:, :table.shape[1]]
+        table[:, :rows.shape[1]] = rows
+        c = mx.KvCache(cache.k, cache.v, table, cache.k_scale, cache.v_scale)
+        if seqs == 250:  # the plain form for some of them
+            q = rand(g, seqs, 2 * group, D)
+            out, lse = torch.empty_like(q), torch.empty(seqs, 2 * group, device="cuda")
+            sl = torch.tensor(lens, device="cuda", dtype=torch.int32)
+            mx.attn_decode_paged(q, c, sl, 2 * group, D ** -0.5, out, lse=lse, workspace=mx.attn_decode_workspace(c, 2 * group))
+            few = list(range(0, seqs, 17))
+            part = mx.KvCache(cache.k, cache.v, table[few].contiguous(), cache.k_scale, cache.v_scale)
+            want = R.decode_reference(q[few], part, [lens[b] for b in few], 2 * group, D ** -0.5, -1, 0)
+            R.assert_within(out[few], want[0], want[2], "out")
+            R.assert_within(lse[few], want[1], want[3], "lse")
+        else:
+            check_decode(mx, 29, kind, lens, 2 * group, 2, D, 16, left=left, sinks=sinks, cache=c)
+
+
 def test_two_streams_at_once(mx):
     """The three calls on two streams at the same time, a workspace each: what they give one after the other."""
     g = gen(60)
