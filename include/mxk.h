@@ -243,8 +243,8 @@ int mxk_linear_gated_residual(const mxk_bf16* A, const mxk_bf16* W, const float*
  * covered; all multiples of 16 bytes, k and v 16-byte aligned).  Token t of sequence b is slot t % page_size of page
  * page_table[b * table_stride + t / page_size]; a sequence has room for max_pages * page_size tokens.  The same page
  * may stand in several rows of the table (a shared prefix).
- * type MXK_KV_BF16: bf16 values.  MXK_KV_E4M3: fp8 e4m3 values, element = value / scale rounded to nearest, ties to
- * even, saturating at +-448; k_scale / v_scale fp32 [Hkv], positive normal numbers, or NULL (1).
+ * type MXK_KV_BF16: bf16 values.  MXK_KV_E4M3: fp8 e4m3 values, element = the fp32 quotient value / scale rounded to
+ * nearest, ties to even, saturating at +-448; k_scale / v_scale fp32 [Hkv], positive normal numbers, or NULL (1).
  * Page numbers, sequence numbers, positions and lengths are read on the device.  One that is out of range is never
  * followed: the row or token is left out and mxk_device_error() reports MXK_DEVICE_ERR_BAD_INDEX. */
 #define MXK_KV_BF16 0

@@ -39,12 +39,25 @@ struct AppendLaunch {
   int* err;
 };
 
-__device__ __forceinline__ uint2 pack8_e4m3(const float* f, float inv_scale) {
+// Eight values / scale as e4m3.  A product with 1 / scale, which is rounded itself, would put quotients that lie exactly between two
+// codes (scales of few significant bits have many) on the wrong side.  So the quotient's remainder, which one fma gives
+// exactly, is divided as well (Markstein, IBM J. Res. Dev. 34, 1990: correctly rounded where the reciprocal is).  Both sides are
+// taken times a power of two that brings the scale into [1, 4), where nothing on the way leaves the normal numbers but quotients that
+// are the code 0.  Saturating, infinite and NaN quotients stay as they are; a zero keeps its sign.  8704 rows of 3 x 24 heads of 128:
+// 71.5 us, with __fdiv_rn 86, with the reciprocal alone 65.
+__device__ __forceinline__ uint2 pack8_e4m3(const float* f, float scale) {
+  const float up = __uint_as_float(0x7f000000u - min(__float_as_uint(scale) & 0x7f800000u, 0x7e800000u));
+  const float m = scale * up, inv = __frcp_rn(m);
   unsigned w[2] = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const __nv_fp8x2_storage_t p = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv_scale, f[2 * i + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3);
-    w[i >> 1] |= unsigned(p) << (16 * (i & 1));
+    float q[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const float x = f[2 * i + e] * up, y = x * inv, rest = fmaf(y, m, -x);
+      q[e] = fabsf(y) < 512.f ? fmaf(rest, -inv, y) : y;
+    }
+    w[i >> 1] |= unsigned(__nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
   }
   return make_uint2(w[0], w[1]);
 }
@@ -194,9 +207,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
       elem* dst = static_cast<elem*>(kind == 1 ? c.k : c.v) + at + int64_t(h) * c.head_stride;
       if (E4M3) {
         const float* sc = kind == 1 ? c.k_scale : c.v_scale;
-        const float inv = sc ? __frcp_rn(sc[h]) : 1.f;
-        *reinterpret_cast<uint2*>(dst + 8 * va) = pack8_e4m3(v, inv);
-        *reinterpret_cast<uint2*>(dst + 8 * vb) = pack8_e4m3(v + 8, inv);
+        const float scale = sc ? sc[h] : 1.f;
+        *reinterpret_cast<uint2*>(dst + 8 * va) = pack8_e4m3(v, scale);
+        *reinterpret_cast<uint2*>(dst + 8 * vb) = pack8_e4m3(v + 8, scale);
       } else {
         *reinterpret_cast<uint4*>(dst + 8 * va) = kind == 2 ? raw[u][0] : pack8_at(v);
         *reinterpret_cast<uint4*>(dst + 8 * vb) = kind == 2 ? raw[u][1] : pack8_at(v + 8);
@@ -322,7 +335,7 @@ __global__ void __launch_bounds__(kAnyThreads) append_any_kernel(const __grid_co
     elem* dst = static_cast<elem*>(is_v ? c.v : c.k) + at + int64_t(g) * c.head_stride + 8 * l;
     if (E4M3) {
       const float* sc = is_v ? c.v_scale : c.k_scale;
-      *reinterpret_cast<uint2*>(dst) = pack8_e4m3(v, sc ? __frcp_rn(sc[g]) : 1.f);
+      *reinterpret_cast<uint2*>(dst) = pack8_e4m3(v, sc ? sc[g] : 1.f);
     } else {
       *reinterpret_cast<uint4*>(dst) = is_v ? raw[u] : pack8(v);
     }

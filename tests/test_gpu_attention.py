@@ -179,6 +179,58 @@ def test_append_without_sequence_numbers_and_saturation(mx):
     assert bool((got.abs()[big & want.isfinite()] == 448).all()) and int(big.sum()) > 100
 
 
+@pytest.mark.parametrize("D, rot", [(64, 64), (128, 128), (80, 40), (48, 6)])
+def test_append_e4m3_is_the_quotient_rounded_once(mx, D, rot):
+    """v and, without a norm and with angles of zero, k: the code nearest to value / scale, of two that are equally near the even
+    one, found by comparing the value with scale * (the middle between two codes), which is exact in 64 bits.  Scales of few bits
+    have many quotients that lie in such a middle."""
+    g = gen(7)
+    scales = [7.0, 3.0, 5.0, 7 / 4096, 11 / 4096, 345 / 4096, 511 / 4096, 0.75]
+    Hkv, T = len(scales), 1500
+    k = torch.zeros(40, 50, Hkv, D, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    sc = torch.tensor(scales, device="cuda")
+    cache = mx.KvCache(k, torch.zeros_like(k.view(torch.uint8)).view(torch.float8_e4m3fn), torch.randperm(40, device="cuda", generator=g).int()[None], sc, sc)
+    # codes of the type in order, the middles between them, and values around those: exact ties where bf16 holds them
+    code = torch.arange(127, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    middle = (code[1:] + code[:-1]) / 2
+    pick = torch.randint(0, 126, (2, T, Hkv, D), device="cuda", generator=g)
+    sign = torch.randint(0, 2, pick.shape, device="cuda", generator=g) * 2 - 1
+    x = (sign * middle[pick] * sc.double()[:, None]).bfloat16()
+    x[:, -100:] = rand(g, 2, 100, Hkv, D, std=30.0) * sc[:, None].bfloat16()
+    q, pos = rand(g, T, D), torch.arange(T, device="cuda", dtype=torch.int32)
+    angle = torch.zeros(T, rot // 2, device="cuda")
+    mx.qkv_norm_rope_append(q, x[0], x[1], T, 1, D, None, None, 1e-6, angle.cos(), angle.sin(), T, rot, 2, cache, pos, torch.empty_like(q),
+                            seq_ids=torch.zeros_like(pos))
+    page, slot = cache.page_table[0].long()[pos.long() // 50], pos.long() % 50
+    ties = 0
+    for t, v in ((cache.k, x[0]), (cache.v, x[1])):
+        a, s = v.double().abs(), sc.double()[:, None]
+        below = (a[..., None] > s[..., None] * middle).sum(-1)  # middles below the value; one equal to it goes to the even code
+        tie = (a[..., None] == s[..., None] * middle).any(-1)
+        want = below + (tie & (below % 2 == 1))
+        got = raw(t)[page, slot].long()
+        assert torch.equal(got & 127, want) and torch.equal(got >> 7, torch.signbit(v).long())
+        ties += int(tie.sum())
+    assert ties > 100000  # the case that the test is about
+
+
+def test_append_e4m3_scales_and_values_at_the_ends_of_fp32(mx):
+    """Every bf16 number under scales from the smallest normal to the largest power of two: the fp32 quotient, rounded."""
+    scales = torch.tensor([2.0 ** -126, 1.75 * 2.0 ** -126, 7 * 2.0 ** -100, 7 * 2.0 ** -64, 1.0, 7 * 2.0 ** 62, 7 * 2.0 ** 100, 1.75 * 2.0 ** 126,
+                           2.0 ** 127, 1.75 * 2.0 ** 127])
+    Hkv, D, T = len(scales), 64, 1024
+    v = torch.arange(1 << 16, dtype=torch.int32).to(torch.uint16).view(torch.bfloat16).view(T, 1, D).expand(T, Hkv, D).contiguous()
+    pages = torch.zeros(2, 16, 64, Hkv, D, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    cache = mx.KvCache(pages[0], pages[1], torch.arange(16, device="cuda", dtype=torch.int32)[None], scales.cuda(), scales.cuda())
+    q, pos, x = torch.zeros(T, D, device="cuda", dtype=torch.bfloat16), torch.arange(T, device="cuda", dtype=torch.int32), v.cuda()
+    mx.qkv_norm_rope_append(q, x, x, T, 1, D, None, None, 1e-6, None, None, 0, 0, 0, cache, pos, torch.empty_like(q), seq_ids=torch.zeros_like(pos))
+    want = (v.float() / scales[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    nan = v.isnan()
+    for t in (cache.k, cache.v):
+        got = raw(t).view(T, Hkv, D).cpu()
+        assert torch.equal(got[~nan], want[~nan]) and bool(((got[nan] & 127) == 127).all())
+
+
 def test_append_bad_indices_are_left_out_and_reported(mx):
     g = gen(6)
     cache = make_cache(mx, g, BF16, 6, 32, 16, 2, 64)
