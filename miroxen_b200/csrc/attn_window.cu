@@ -40,6 +40,7 @@
 #include "bulk_copy.cuh"
 #include "common.cuh"
 #include "kv_cache.cuh"
+#include "tuning.h"
 
 namespace mxk {
 namespace {
@@ -286,6 +287,7 @@ struct WindowLaunch {
   AttnLaunch L;
   int halves;     // 128-row halves of a tile: 2, or 1 where that leaves SMs idle
   int max_tiles;  // the grid has max_tiles * H CTAs
+  int reversed;   // 1: the numbers of tiles fall with those of the CTAs
 };
 
 // What a tile is: rows [r0, r0 + rows) and head `head` of a sequence that starts at row q0 / key k0 and has nq rows, nk keys.
@@ -301,8 +303,9 @@ struct TileSearch {
 
 // Tile number `cta` of the launch, by one warp; rows = 0 if there is no such tile.  Counted from the back: the tiles at the end
 // of a causal sequence, which have the most keys, come first, all heads of a tile one behind the other (the other way round,
-// head by head, the CTAs at work crowd on the same few lines of the keys: packed prompts 195 against 145 us).  Numbers never
-// fall from one search of a CTA to its next, so that each goes on where the last one ended.
+// head by head, the CTAs at work crowd on the same few lines of the keys: packed prompts 195 against 145 us).  A search goes on
+// where the CTA's last one ended; where the hardware hands out a number from in front of that (nothing promises an order), it
+// starts again.
 __device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta, TileSearch& from) {
   const MxkAttnArgs& a = W.L.a;
   const int lane = threadIdx.x & 31, tile_rows = kM * W.halves, place = cta / a.H;
@@ -312,6 +315,7 @@ __device__ __forceinline__ WindowTile find_tile(const WindowLaunch& W, int cta, 
     t.rows = min(tile_rows, t.nq - t.r0);
     return t;
   }
+  if (place < from.tiles) from = TileSearch{};
   constexpr int kAhead = 4;  // groups of 32 sequences whose ends are asked for at once
   for (; from.seqs < a.n_seqs; from.seqs += 32 * kAhead) {
     int x[kAhead][4];
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
       int cta = int(blockIdx.x), n = 0;
       TileSearch search;
       for (int asks = 0; ok; asks++) {
-        t = find_tile(W, cta, search);
+        t = find_tile(W, W.reversed ? int(gridDim.x) - 1 - cta : cta, search);
         if (t.rows > 0) {
           if (n >= 2) ok = wait(&sm.tile_empty[n & 1], (n >> 1) - 1);
           if (ok && leader) {
@@ -908,7 +912,7 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   L.left = a.left < 0 || a.left > kFar ? kFar : int(a.left);
   L.right = a.right < 0 || a.right > kFar ? kFar : int(a.right);
   L.sinks = a.sinks > kFar ? kFar : int(a.sinks);
-  WindowLaunch W{L, 2, 0};
+  WindowLaunch W{L, 2, 0, tune(TUNE_WINDOW_ORDER, 1) == 2};
   // at most one tile per sequence is not full
   auto tiles = [&](int rows) { return a.n_seqs == 1 ? ceil_div(a.q_rows, rows) : a.q_rows / rows + (a.n_seqs < a.q_rows ? a.n_seqs : a.q_rows); };
   if (tiles(2 * kM) * a.H <= sm_count() / 2) W.halves = 1;  // twice the CTAs still fit the GPU at once

@@ -37,6 +37,7 @@ enum TuneKey {
   TUNE_ROPE_WIDE_REGS,     // wide head kernel's register budget: 1 = 128 registers for CTAs of up to 128 threads (default), 2 = 96 everywhere
   TUNE_LINEAR_CTAS,        // linear layers: 2 = a pair of CTAs per 256 x 256 tile, 1 = one CTA per 128 x 256 tile, 0 = whichever needs fewer waves (default)
   TUNE_LINEAR_GROUP_M,     // linear layers: row tiles per band of the tile order (default 8 for CTA pairs, 16 for single CTAs)
+  TUNE_WINDOW_ORDER,       // attn_window: 1 tiles from the back of the batch (default), 2 from its front
   TUNE_COUNT
 };
 

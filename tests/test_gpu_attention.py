@@ -537,6 +537,23 @@ def test_window_thousands_of_sequences(mx):
     check_window(mx, 36, [1] * 700, [1] * 700, 2, 1, 128, 3, 0, 1, behind=5)
 
 
+@pytest.fixture(params=[1, 2], ids=["from_the_back", "from_the_front"])
+def order(mx, request):
+    mx.set_tuning("window_order", request.param)
+    yield request.param
+    mx.set_tuning("window_order", 0)
+
+
+def test_window_tiles_in_either_order(mx, order):
+    """Many more tiles than CTAs at a time, looked for in rising and in falling order, with searches past the first sequences and
+    numbers that no tile has: every row is computed once whatever order the tiles come in."""
+    rng = random.Random(10)
+    rows = [rng.choice([0, 1, 3, 40, 129, 300]) for _ in range(400)]
+    check_window(mx, 51, rows, rows, 4, 2, 64, -1, 0, 0, behind=9)
+    check_window(mx, 52, [1] * 900, [2] * 900, 2, 1, 128, 3, 0, 1)
+    check_window(mx, 53, [9000], [9000], 8, 2, 64, 200, 0, 3, cu=False)
+
+
 def test_window_scores_that_grow_along_the_keys(mx):
     """Every block of keys has a larger maximum than the one in front of it, by more and by less than a factor of 2^8."""
     def edit(q, k, v):
