@@ -321,7 +321,9 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args_host, const MxkKvCache* cach
  *   j >= p - left or j < sinks  (left < 0: no bound)
  * out[i, h] = sum_j softmax_j(scale * q[i, h] . k_j) v_j; lse fp32 [q_rows, H] or NULL as above.  A row that sees
  * nothing gives out 0 and lse -inf; rows of q and out that belong to no sequence are left as they were, and k / v rows
- * that belong to no sequence, or lie outside of every row's view, do not reach any output whatever they hold.
+ * that belong to no sequence, or lie outside of every row's view, do not reach any output whatever they hold.  (Where v rows
+ * within 128 keys of the edge of a row's view are not finite, that row is taken again one key at a time, hundreds of times slower:
+ * zero the rows of v between and behind the sequences where speed counts.)
  * q, k, v, out: bf16, head h of a row at row * stride + h * D; strides multiples of 8, pointers 16-byte aligned;
  * head h reads key head h / (H / Hkv); D a multiple of 8, at most 128; fewer than 2^30 rows; 0 < scale <= 1e30.  out
  * overlaps no input. */

@@ -288,6 +288,7 @@ struct WindowLaunch {
   int halves;     // 128-row halves of a tile: 2, or 1 where that leaves SMs idle
   int max_tiles;  // the grid has max_tiles * H CTAs
   int reversed;   // 1: the numbers of tiles fall with those of the CTAs
+  unsigned tries;  // of a wait
 };
 
 // What a tile is: rows [r0, r0 + rows) and head `head` of a sequence that starts at row q0 / key k0 and has nq rows, nk keys.
@@ -477,8 +478,9 @@ __global__ void __launch_bounds__(kThreadsW, 1)
 
   // Every wait is bounded; a role whose wait runs out leaves its loop, the others' waits then run out too.
   bool ok = true;
+  auto lane_wait = [&](unsigned long long* bar, int phase) { return mbar_wait_spin(smem_u32(bar), unsigned(phase) & 1u, W.tries); };
   auto wait = [&](unsigned long long* bar, int phase) {
-    const bool r = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(bar), unsigned(phase) & 1u));
+    const bool r = __all_sync(0xffffffffu, lane_wait(bar, phase));
     fence_after();
     return r;
   };
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         if (!(block <= last && (block < sinks || block >= from))) continue;
         const bool edge = !(block < full_to && (block >= full_from || block < full_sinks));
         // A wait that runs out: the warp goes on without waiting for anything else.  Its lanes agree on the outcome.
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.s_full[h]), unsigned(all) & 1u));
+        ok = ok && __all_sync(0xffffffffu, lane_wait(&sm.s_full[h], all));
         fence_after();
         unsigned s[4][32];
 #pragma unroll
@@ -699,7 +701,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
             m = mx, l *= f;
           }
           if (done > 0 && ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u));
+            ok = __all_sync(0xffffffffu, lane_wait(&sm.pv_done[h], all - 1));
             fence_after();
 #pragma unroll 1
             for (int c = 0; c < DP / 16; c++) {
@@ -719,7 +721,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
           unsigned p[16];
           exp_chunk(s[c], scale2, neg_base, l2, p);
           if (c == 0 && done > 0 && ok) {  // P is the product's until it has retired
-            ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u));
+            ok = __all_sync(0xffffffffu, lane_wait(&sm.pv_done[h], all - 1));
             fence_after();
           }
           tmem_st16(tp + 16 * c, p);
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(kThreadsW, 1)
         done++, all++;
       }
       // ---- output ----
-      if (ok && done > 0) ok = mbar_wait_spin(smem_u32(&sm.pv_done[h]), unsigned(all - 1) & 1u);
+      if (ok && done > 0) ok = lane_wait(&sm.pv_done[h], all - 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
@@ -912,7 +914,12 @@ extern "C" int mxk_attn_window(const MxkAttnArgs* args, mxk_stream_t stream) {
   L.left = a.left < 0 || a.left > kFar ? kFar : int(a.left);
   L.right = a.right < 0 || a.right > kFar ? kFar : int(a.right);
   L.sinks = a.sinks > kFar ? kFar : int(a.sinks);
-  WindowLaunch W{L, 2, 0, tune(TUNE_WINDOW_ORDER, 1) == 2};
+  WindowLaunch W{L, 2, 0, tune(TUNE_WINDOW_ORDER, 1) == 2, 0u};
+  // What a warp may have to wait for grows with the keys: up to 32 rows taken again by one warp, each 32 keys at a time, are as many
+  // steps as there are keys, 4.6 us each measured, 15.6 us with all warps of the GPU at it (30000 keys of 128 channels: 139 and
+  // 469 ms a tile); and with the sequences that a search passes, 128 at a time.  128 tries are twelve times such a step.
+  const int64_t tries = tune(TUNE_WINDOW_WAIT_TRIES, int(kSpinTries)) + 128 * a.k_rows + a.n_seqs;
+  W.tries = unsigned(tries < 0xffffffffll ? tries : 0xffffffffll);
   // at most one tile per sequence is not full
   auto tiles = [&](int rows) { return a.n_seqs == 1 ? ceil_div(a.q_rows, rows) : a.q_rows / rows + (a.n_seqs < a.q_rows ? a.n_seqs : a.q_rows); };
   if (tiles(2 * kM) * a.H <= sm_count() / 2) W.halves = 1;  // twice the CTAs still fit the GPU at once

@@ -48,10 +48,10 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity) {
   return false;
 }
 // The same without the sleeps and with the phase looked at first, for hand-overs between warps that happen every
-// microsecond or less and have mostly happened when they are waited for.
+// microsecond or less and have mostly happened when they are waited for.  A try takes up to 1.5 us.
 constexpr unsigned kSpinTries = 1u << 22;
-__device__ __forceinline__ bool mbar_wait_spin(unsigned bar, unsigned parity) {
-  for (unsigned i = 0; i < kSpinTries; i++) {
+__device__ __forceinline__ bool mbar_wait_spin(unsigned bar, unsigned parity, unsigned tries = kSpinTries) {
+  for (unsigned i = 0; i < tries; i++) {
     unsigned ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"

@@ -38,6 +38,7 @@ enum TuneKey {
   TUNE_LINEAR_CTAS,        // linear layers: 2 = a pair of CTAs per 256 x 256 tile, 1 = one CTA per 128 x 256 tile, 0 = whichever needs fewer waves (default)
   TUNE_LINEAR_GROUP_M,     // linear layers: row tiles per band of the tile order (default 8 for CTA pairs, 16 for single CTAs)
   TUNE_WINDOW_ORDER,       // attn_window: 1 tiles from the back of the batch (default), 2 from its front
+  TUNE_WINDOW_WAIT_TRIES,  // attn_window: tries of a wait between its warps, 1.5 us each, before it counts as run out (default 2^22), beside those that long views add
   TUNE_COUNT
 };
 

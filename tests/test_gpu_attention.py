@@ -577,6 +577,19 @@ def test_window_rows_of_nobody_may_hold_anything(mx):
     check_window(mx, 41, [100], [700], 2, 1, 128, 99, 0, 10, edit=unseen)
 
 
+def test_window_rows_taken_again_outlast_a_wait(mx):
+    """Values behind the last key that are not finite: every row is taken again by a loop over its keys, 20 ms a tile, and the CTAs'
+    next tiles stand behind that.  A wait between warps, here of 3 ms and what the keys add to it, must not run out meanwhile."""
+    def edit(q, k, v):
+        k[4000:], v[4000:] = float("nan"), float("inf")
+    mx.set_tuning("window_wait_tries", 1 << 11)
+    try:
+        check_window(mx, 54, [64], [4000], 160, 1, 64, behind=20, edit=edit)
+        check_window(mx, 55, [33, 31], [2000, 4000 - 2000], 90, 2, 128, behind=1, edit=edit)
+    finally:
+        mx.set_tuning("window_wait_tries", 0)
+
+
 @pytest.mark.parametrize("what", ["nan", "inf"])
 def test_window_values_reach_only_rows_that_see_them(mx, what):
     """A NaN or an infinity in the values of one key: rows that do not see the key are as they would be without it."""
