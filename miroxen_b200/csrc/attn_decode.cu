@@ -93,10 +93,15 @@ __device__ __forceinline__ View view_of(const DecodeLaunch& p, int b) {
   return v;
 }
 
+// Tiles of `len` tokens; 31 bits hold the tokens, but not their number rounded up.
+template <int TILE>
+__device__ __forceinline__ int tiles_in(int len) {
+  return int((unsigned(len) + TILE - 1) / TILE);
+}
 // Tiles of sequence b, all its work items.
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const DecodeLaunch& p, int b) {
-  return (view_of(p, b).len + TILE - 1) / TILE * p.heads;
+  return tiles_in<TILE>(view_of(p, b).len) * p.heads;
 }
 
 // Finds, with the whole CTA: the number of tiles of the call, and for tile `want` of the caller's choosing (a function of
@@ -149,7 +154,7 @@ template <int TILE>
 __device__ __forceinline__ void cursor_sequence(const DecodeLaunch& p, Cursor& c) {  // sequences without a token are passed over
   while (c.b < p.c.n_seqs) {
     c.v = view_of(p, c.b);
-    c.n_tiles = (c.v.len + TILE - 1) / TILE;
+    c.n_tiles = tiles_in<TILE>(c.v.len);
     if (c.n_tiles > 0) return;
     c.b++;
   }
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
     const int item = int(blockIdx.x) / p.cluster, rank = int(blockIdx.x) - item * p.cluster;
     cur.b = item / p.heads, cur.head = item - cur.b * p.heads;
     cur.v = view_of(p, cur.b);
-    cur.n_tiles = (cur.v.len + kTile - 1) / kTile;
+    cur.n_tiles = tiles_in<kTile>(cur.v.len);
     const int lo = rank * cur.n_tiles / p.cluster;
     n_my = (rank + 1) * cur.n_tiles / p.cluster - lo;
     cur.tile = cur.lo = lo, cur.hi = lo + n_my, cur.left = n_my, cur.rest = 0;
@@ -340,10 +345,10 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       head_off = int64_t(cur.head / p.blocks) * p.c.head_stride;
 #pragma unroll
       for (int x = 0; x < kPL; x++) {
-        const int i = cur.tile * kTile + (part * kPL + x) * 32 + lane;
+        const unsigned i = unsigned(cur.tile) * kTile + unsigned((part * kPL + x) * 32 + lane);  // may pass 31 bits, in the last tile
         page[x] = 0, slot[x] = -1;
-        if (i < cur.v.len) {  // inside the table: the length is held to it
-          const int tok = i < cur.v.first ? i : i - cur.v.first + cur.v.skip;
+        if (i < unsigned(cur.v.len)) {  // inside the table: the length is held to it
+          const int tok = int(i < unsigned(cur.v.first) ? i : i - unsigned(cur.v.first) + unsigned(cur.v.skip));
           // tok / page_size by the reciprocal rounded down, at most one too small for tok < 2^31
           int n = int(__umulhi(unsigned(tok), p.page_recip)), r = tok - n * p.c.page_size;
           if (r >= p.c.page_size) n++, r -= p.c.page_size;
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(kConsumers) join_kernel(const __grid_constant_
   if (lane == 0) sums[0][warp] = total, sums[1][warp] = before;
   __syncthreads();
   total = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3], before = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-  const int n_tiles = (view_of(p, b).len + TILE - 1) / TILE;
+  const int n_tiles = tiles_in<TILE>(view_of(p, b).len);
   if (n_tiles == 0) return;
   const int per = (total + p.ctas - 1) / p.ctas;
   const int s0 = before + head * n_tiles, c0 = s0 / per, c1 = (s0 + n_tiles - 1) / per;

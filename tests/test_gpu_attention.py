@@ -416,6 +416,31 @@ def test_decode_offsets_past_32_bits(mx):
     torch.cuda.empty_cache()
 
 
+def test_decode_the_longest_sequence(mx):
+    """2^31 - 2 tokens, all but the last few in one page that the table names again and again: keys of zero and values of one, so that
+    every sum is a whole number of 2^7 below 2^24 of them in a run, and fp32 holds it; the second sequence ends in a page whose
+    last key outweighs all others (e^40 against 2^31 < e^22)."""
+    page, pages, D = 32767, 65538, 16
+    kv = torch.zeros(2, 2, page, 1, D, device="cuda")
+    kv[1] = 1.0
+    kv[0, 1, -1], kv[1, 1, -1] = 2.5, -2.0
+    kv = kv.to(torch.float8_e4m3fn)
+    table = torch.zeros(2, pages, dtype=torch.int32, device="cuda")
+    table[1, -1] = 1
+    cache = mx.KvCache(kv[0], kv[1], table)
+    n = page * pages
+    assert n == 2 ** 31 - 2
+    q, lens = torch.ones(2, 1, D, device="cuda", dtype=torch.bfloat16), torch.full((2,), n, dtype=torch.int32, device="cuda")
+    ws = mx.attn_decode_workspace(cache, 1)
+    for left, sinks in ((-1, 0), (n - 2, 1), (1000, 3)):
+        out, lse = torch.full_like(q, 7.0), torch.full((2, 1), 7.0, device="cuda")
+        mx.attn_decode_paged(q, cache, lens, 1, 1.0, out, left=left, sinks=sinks, lse=lse, workspace=ws)
+        seen = n if left < 0 else min(n, left + 1 + sinks)
+        assert bool((out[0] == 1).all()) and bool((out[1] == -2).all())
+        want = torch.tensor([math.log(seen), 40 + math.log1p(seen * math.exp(-40))])
+        assert float((lse.cpu()[:, 0].double() - want).abs().max()) <= 2.0 ** -18  # steps of 2^-22 near 21 and 40, log2 and exp2 to 2^-22
+
+
 @pytest.mark.parametrize("kind", [BF16, E4M3])
 def test_decode_many_small_weights(mx, kind):
     """A million tokens of weight 2^-25.1 behind one of weight 1, as many work items as fill the GPU with such runs: what the
