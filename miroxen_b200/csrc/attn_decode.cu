@@ -879,6 +879,7 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   if (int rc = check_cache(name, cache)) return rc;
   if (cache->n_seqs <= 0) return MXK_OK;
   if (int rc = check_heads(name, cache, args->H)) return rc;
+  if (cache->max_pages > 0 && !cache->page_table) return fail(MXK_ERR_INVALID_ARG, "%s: null page table", name);
   if (cache->max_pages > 0 && cache->num_pages > 0)
     if (int rc = check_cache_pointers(name, cache)) return rc;
   DecodeLaunch p{};
@@ -890,6 +891,8 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
     return fail(MXK_ERR_INVALID_ARG, "%s: q, out and workspace must be 16-byte aligned", name);
   if (a.sinks < 0) return fail(MXK_ERR_INVALID_ARG, "%s: sinks=%lld", name, (long long)a.sinks);
   if (!(a.scale > 0.f) || a.scale > 1e30f) return fail(MXK_ERR_INVALID_ARG, "%s: scale must be positive and at most 1e30", name);
+  // without a page every token is left out; the copies of no bytes that stand for it then have an address that exists
+  if (cache->num_pages == 0) p.c.k = p.c.v = const_cast<mxk_bf16*>(a.q);
   p.group = a.H / cache->Hkv;
   p.blocks = int(ceil_div(p.group, 16));
   p.heads = cache->Hkv * p.blocks;

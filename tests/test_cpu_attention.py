@@ -110,6 +110,13 @@ def test_decode_null_structs_and_noops(L):
     assert lib.mxk_attn_decode_workspace_bytes(cache(L), 12) == -1
 
 
+def test_decode_needs_a_page_table_wherever_it_may_look_into_it(L):
+    lib = L.lib()
+    for more in (dict(), dict(num_pages=0), dict(num_pages=0, k=None, v=None), dict(num_pages=0, type=1)):
+        assert lib.mxk_attn_decode_paged(decode(L), cache(L, page_table=None, **more), None) == -1
+        assert b"attn_decode_paged" in lib.mxk_last_error() and b"page table" in lib.mxk_last_error()
+
+
 @pytest.mark.parametrize("bad", [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=P + 2), dict(k=P + 8), dict(v=P + 4),
                                  dict(out=P + 8), dict(k_rows=-1), dict(H=0), dict(Hkv=0), dict(H=12), dict(D=4), dict(D=130), dict(D=136),
                                  dict(cu_q=None), dict(cu_k=None), dict(cu_q=None, cu_k=None), dict(q_stride=4092), dict(q_stride=4088),

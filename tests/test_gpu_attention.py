@@ -392,6 +392,20 @@ def test_decode_bad_pages_and_lengths_are_left_out_and_reported(mx):
     assert bool((out[3] == 0).all()) and torch.equal(out[0], good[0])
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_decode_without_a_page(mx, kind):
+    """A cache of no pages at all: every token is left out and reported, whatever the table says."""
+    empty = torch.zeros(2, 0, 16, 2, 64, device="cuda", dtype=torch.bfloat16 if kind == BF16 else torch.uint8)
+    empty = empty if kind == BF16 else empty.view(torch.float8_e4m3fn)
+    cache = mx.KvCache(empty[0], empty[1], torch.tensor([[0, 1], [-1, 5]], device="cuda", dtype=torch.int32))
+    q, lse = rand(gen(30), 2, 4, 64), torch.full((2, 4), 7.0, device="cuda")
+    out = torch.full_like(q, 7.0)
+    mx.attn_decode_paged(q, cache, torch.tensor([20, 32], device="cuda", dtype=torch.int32), 4, 0.125, out, lse=lse, workspace=mx.attn_decode_workspace(cache, 4))
+    torch.cuda.synchronize()
+    assert mx.device_error() == 2
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
 def test_decode_refuses_a_small_workspace(mx):
     g = gen(24)
     cache = make_cache(mx, g, BF16, 2, 4000, 16, 2, 128)
