@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 import re
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -77,6 +78,24 @@ class AttnArgs(C.Structure):
                 ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("out_stride", C.c_int64), ("left", C.c_int64),
                 ("right", C.c_int64), ("sinks", C.c_int64), ("n_seqs", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32),
                 ("D", C.c_int32), ("scale", C.c_float)]
+
+
+_CODES = {C.c_void_p: "Q", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+
+
+def maker(cls):
+    """cls(...) from all its fields' values in their order, null pointers as 0, without a conversion per field (0.4 instead of
+    1.3 us for the twenty-one of AppendArgs); a value that its field cannot hold is an MxkError."""
+    layout = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_) + "0Q")
+    assert layout.size == C.sizeof(cls)
+    pack, copy = layout.pack, cls.from_buffer_copy
+
+    def make(*values):
+        try:
+            return copy(pack(*values))
+        except (struct.error, OverflowError) as e:
+            raise MxkError(f"{cls.__name__}: {e}") from None
+    return make
 
 
 _P, _I64, _I, _F = C.c_void_p, C.c_int64, C.c_int, C.c_float

@@ -7,6 +7,7 @@ stream.  Every function launches asynchronously and raises MxkError on a non-zer
 from __future__ import annotations
 
 import ctypes as C
+import sys
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -14,11 +15,13 @@ import torch
 
 from . import _lib
 from ._lib import (AppendArgs, AttnArgs, BlockArgs, DecodeArgs, HeadTensor, KvCacheArgs, MxkError, RopeRun, RowMod, check,
-                   lib)
+                   lib, maker)
 
 ROPE_NONE, ROPE_INTERLEAVED, ROPE_HALF = 0, 1, 2
 ACT_GELU_TANH, ACT_SILU_MUL, ACT_GELU_ERF = 0, 1, 2
 KV_BF16, KV_E4M3 = 0, 1
+_append_args, _decode_args, _attn_args = maker(AppendArgs), maker(DecodeArgs), maker(AttnArgs)
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 Q_MXFP8, Q_NVFP4 = 1, 2  # QMode of src/kernels/blockscale.h:14 (0 = None is not a quantised mode)
 
 __all__ = [
@@ -364,15 +367,32 @@ class KvCache:
                                  k.shape[2], k.shape[3], KV_BF16 if k.dtype == torch.bfloat16 else KV_E4M3)
 
 
-def _here(what, index, stream=None):
-    """The library works on the current device; a tensor of another one (of index `index`, -1: none) is refused before its
-    address gets there.  Returns the handle of the stream the call goes to."""
+def _here(stream=None):
+    """(index of the current device, which the library works on; handle of the stream the call goes to)"""
     now = torch.cuda.current_device()
-    if index >= 0 and index != now:
-        raise MxkError(f"{what}: tensors on cuda:{index}, but the current device is cuda:{now}")
     if stream is None and _raw_stream is not None:
-        return _raw_stream(now) or None
-    return _stream(stream)
+        return now, _raw_stream(now) or None
+    return now, _stream(stream)
+
+
+def _at(t, dtype, now):
+    """The address of a tensor that has to be of this type and on the current device, before it gets there; integers are addresses
+    of the caller's own."""
+    try:
+        if t.dtype is dtype and t.get_device() == now:
+            return t.data_ptr()
+    except AttributeError:
+        return t
+    return _elsewhere(t, dtype, now)
+
+
+def _elsewhere(t, dtype, now):
+    what = next(f.f_code.co_name for f in (sys._getframe(1), sys._getframe(2)) if f.f_code is not _at.__code__)
+    if t.dtype is not dtype:
+        raise MxkError(f"{what}: a tensor {list(t.shape)} of {t.dtype}, where {dtype} belongs")
+    if t.device.type != "cpu" or not t.is_pinned():  # pinned host memory is the device's as well
+        raise MxkError(f"{what}: a tensor {list(t.shape)} on {t.device}, but the current device is cuda:{now}")
+    return t.data_ptr()
 
 
 def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, table_rows, rot, mode, cache: KvCache, positions,
@@ -381,18 +401,25 @@ def qkv_norm_rope_append(q, k, v, T, H, D, q_norm_w, k_norm_w, eps, cos, sin, ta
     c = cache._args
     if D != c.D:
         raise MxkError(f"qkv_norm_rope_append: D={D} and a cache of D={c.D}")
-    handle = _here("qkv_norm_rope_append", cache._index, stream)
+    now, handle = _here(stream)
+    if cache._index != now:
+        _elsewhere(cache.k, cache.k.dtype, now)
     kv = c.Hkv * D
-    a = AppendArgs(_p(q), _p(k), _p(v), T, H * D if q_stride is None else q_stride, kv if k_stride is None else k_stride,
-                   kv if v_stride is None else v_stride, _p(q_norm_w), _p(k_norm_w), _p(cos), _p(sin), table_rows, _p(positions),
-                   _p(seq_ids), _p(rope_rows), _p(q_out), _p(k_out), H, rot, mode, eps)
+    a = _append_args(_at(q, _BF16, now), _at(k, _BF16, now), _at(v, _BF16, now), T, H * D if q_stride is None else q_stride,
+                     kv if k_stride is None else k_stride, kv if v_stride is None else v_stride, 0 if q_norm_w is None else _at(q_norm_w, _F32, now),
+                     0 if k_norm_w is None else _at(k_norm_w, _F32, now), 0 if cos is None else _at(cos, _F32, now),
+                     0 if sin is None else _at(sin, _F32, now), table_rows, _at(positions, _I32, now), 0 if seq_ids is None else _at(seq_ids, _I32, now),
+                     0 if rope_rows is None else _at(rope_rows, _I32, now), _at(q_out, _BF16, now), 0 if k_out is None else _at(k_out, _BF16, now), H, rot,
+                     mode, eps)
     check(lib().mxk_qkv_norm_rope_append(a, c, handle))
 
 
 def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
     """Scratch memory for attn_decode_paged with this cache and head count, allocated on the current stream: keep one for
     each stream or graph that may run at the same time as another."""
-    _here("attn_decode_workspace", cache._index)
+    now = torch.cuda.current_device()
+    if cache._index != now:
+        _elsewhere(cache.k, cache.k.dtype, now)
     n = lib().mxk_attn_decode_workspace_bytes(cache._args, H)
     if n < 0:
         check(n)
@@ -402,8 +429,11 @@ def attn_decode_workspace(cache: KvCache, H) -> torch.Tensor:
 def attn_decode_paged(q, cache: KvCache, seq_lens, H, scale, out, left=-1, sinks=0, q_stride=None, lse=None, *, workspace, stream=None):
     """Attention of one new token of every sequence over its tokens in the cache."""
     c = cache._args
-    handle = _here("attn_decode_paged", cache._index, stream)
-    a = DecodeArgs(_p(q), H * c.D if q_stride is None else q_stride, _p(seq_lens), _p(out), _p(lse), _p(workspace), workspace.nbytes, left, sinks, H, scale)
+    now, handle = _here(stream)
+    if cache._index != now:
+        _elsewhere(cache.k, cache.k.dtype, now)
+    a = _decode_args(_at(q, _BF16, now), H * c.D if q_stride is None else q_stride, _at(seq_lens, _I32, now), _at(out, _BF16, now),
+                     0 if lse is None else _at(lse, _F32, now), _at(workspace, workspace.dtype, now), workspace.nbytes, left, sinks, H, scale)
     check(lib().mxk_attn_decode_paged(a, c, handle))
 
 
@@ -413,10 +443,13 @@ def attn_window(q, k, v, q_rows, k_rows, H, Hkv, D, scale, out, left=-1, right=-
     window of `left` / `right` keys (-1: no bound; right = 0: causal) and `sinks` first keys that stay visible."""
     if n_seqs is None:
         n_seqs = 1 if cu_q is None else cu_q.numel() - 1
-    handle = _here("attn_window", -1 if q.__class__ is int else q.get_device(), stream)
-    a = AttnArgs(_p(q), _p(k), _p(v), _p(out), _p(lse), _p(cu_q), _p(cu_k), q_rows, k_rows, H * D if q_stride is None else q_stride,
-                 Hkv * D if k_stride is None else k_stride, Hkv * D if v_stride is None else v_stride,
-                 H * D if out_stride is None else out_stride, left, right, sinks, n_seqs, H, Hkv, D, scale)
+        if cu_k is not None and cu_k.__class__ is not int and cu_k.numel() != n_seqs + 1:
+            raise MxkError(f"attn_window: cu_q and cu_k of {n_seqs + 1} and {cu_k.numel()} numbers")
+    now, handle = _here(stream)
+    a = _attn_args(_at(q, _BF16, now), _at(k, _BF16, now), _at(v, _BF16, now), _at(out, _BF16, now), 0 if lse is None else _at(lse, _F32, now),
+                   0 if cu_q is None else _at(cu_q, _I32, now), 0 if cu_k is None else _at(cu_k, _I32, now), q_rows, k_rows,
+                   H * D if q_stride is None else q_stride, Hkv * D if k_stride is None else k_stride, Hkv * D if v_stride is None else v_stride,
+                   H * D if out_stride is None else out_stride, left, right, sinks, n_seqs, H, Hkv, D, scale)
     check(lib().mxk_attn_window(a, handle))
 
 

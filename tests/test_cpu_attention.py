@@ -165,6 +165,60 @@ def test_cache_handle_checks_its_tensors(L):
         mx.qkv_norm_rope_append(P, P, P, 1, 2, 128, None, None, 1e-6, None, None, 0, 0, 0, mx.KvCache(k, k.clone(), table), P, P)
 
 
+def test_tensors_of_another_type_or_place_never_reach_the_library(L, monkeypatch):
+    """Every tensor of each call in turn on the host, or of another type: refused by name, before its address goes anywhere."""
+    import miroxen_b200 as mx
+    from miroxen_b200 import ops
+
+    class Reached:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} was reached")
+
+    class OnGpu(torch.Tensor):  # says that it is on the current device
+        def get_device(self):
+            return 0
+
+    def on(t):
+        return t.as_subclass(OnGpu)
+
+    monkeypatch.setattr(ops, "lib", lambda: Reached())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda i: 0)
+    bf = torch.zeros(4, 256, dtype=torch.bfloat16)
+    f, i = torch.zeros(4, 64), torch.zeros(5, dtype=torch.int32)
+    pages, table = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 3, dtype=torch.int32)
+    cache = mx.KvCache(pages, pages, table)
+    cache._index = 0
+    calls = {
+        "qkv_norm_rope_append": (lambda a: mx.qkv_norm_rope_append(a["q"], a["k"], a["v"], 4, 4, 64, a["qw"], a["kw"], 1e-6, a["cos"], a["sin"], 4, 64, 2, cache,
+                                                                   a["pos"], a["q_out"], seq_ids=a["ids"], rope_rows=a["rows"], k_out=a["k_out"]),
+                                 dict(q=bf, k=bf, v=bf, qw=f, kw=f, cos=f, sin=f, pos=i, q_out=bf, ids=i, rows=i, k_out=bf)),
+        "attn_decode_paged": (lambda a: mx.attn_decode_paged(a["q"], cache, a["lens"], 4, 0.1, a["out"], lse=a["lse"], workspace=a["ws"]),
+                              dict(q=bf, lens=i, out=bf, lse=f, ws=torch.zeros(64, dtype=torch.uint8))),
+        "attn_window": (lambda a: mx.attn_window(a["q"], a["k"], a["v"], 4, 4, 4, 4, 64, 0.1, a["out"], cu_q=a["cu_q"], cu_k=a["cu_k"], lse=a["lse"]),
+                        dict(q=bf, k=bf, v=bf, out=bf, cu_q=i, cu_k=i, lse=f))}
+    for name, (call, tensors) in calls.items():
+        good = {k: on(t) for k, t in tensors.items()}
+        with pytest.raises(AssertionError, match="was reached"):
+            call(good)
+        for k, t in tensors.items():
+            with pytest.raises(mx.MxkError, match=f"{name}: .* on cpu"):
+                call({**good, k: t})
+            if k != "ws":
+                with pytest.raises(mx.MxkError, match=f"{name}: .*{str(t.dtype)[6:]} belongs"):
+                    call({**good, k: on(t.to(torch.int64 if t.dtype == torch.int32 else torch.float16))})
+    cache._index = 1
+    for name in ("qkv_norm_rope_append", "attn_decode_paged"):
+        with pytest.raises(mx.MxkError, match=f"{name}: .* current device is cuda:0"):
+            calls[name][0]({k: on(t) for k, t in calls[name][1].items()})
+    with pytest.raises(mx.MxkError, match="attn_decode_workspace: .* current device is cuda:0"):
+        mx.attn_decode_workspace(cache, 4)
+    with pytest.raises(mx.MxkError, match="cu_q and cu_k"):
+        mx.attn_window(on(bf), on(bf), on(bf), 4, 4, 4, 4, 64, 0.1, on(bf), cu_q=on(i), cu_k=on(i[:4]))
+    with pytest.raises(mx.MxkError, match="AttnArgs"):
+        mx.attn_window(on(bf), on(bf), on(bf), 4, 4, 1 << 32, 4, 64, 0.1, on(bf))
+
+
 def test_plain_forms_of_the_benchmark_agree_with_the_reference():
     """The bounds of attention_ref hold for a softmax in 32 bits rounded once, and not for a wrong window."""
     import attention_ref as R

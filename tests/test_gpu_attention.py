@@ -760,6 +760,24 @@ def test_a_prompt_and_then_single_tokens(mx, kind):
                 assert bool(((o1[b].double() - ref[0][0]).norm(dim=1) <= ref[0][0].norm(dim=1) + 4).all()) and bool(size.isfinite().all())
 
 
+def test_tensors_of_another_place_or_type_are_refused(mx):
+    """Host tensors and 64-bit lengths are refused; pinned host memory, which the device reads, is not."""
+    g = gen(31)
+    cache = make_cache(mx, g, BF16, 2, 40, 16, 2, 64)
+    q, lens = rand(g, 2, 4, 64), torch.tensor([40, 7], dtype=torch.int32)
+    ws, outs = mx.attn_decode_workspace(cache, 4), []
+    for t in (lens.cuda(), lens.pin_memory()):
+        outs.append(torch.empty_like(q))
+        mx.attn_decode_paged(q, cache, t, 4, 0.125, outs[-1], workspace=ws)
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
+    for bad in (lens, lens.cuda().long()):
+        with pytest.raises(mx.MxkError, match="attn_decode_paged"):
+            mx.attn_decode_paged(q, cache, bad, 4, 0.125, outs[0], workspace=ws)
+    with pytest.raises(mx.MxkError, match="attn_window: .* on cpu"):
+        mx.attn_window(q, q.cpu(), q, 2, 2, 4, 4, 64, 0.125, outs[0])
+
+
 @pytest.mark.parametrize("kind", [BF16, E4M3])
 def test_decode_wide_tables_and_short_sequences(mx, kind):
     """Tables with room for far more tokens than there are (the call cannot know), and the same lengths in tables that just
