@@ -145,3 +145,12 @@ int main() {
     assert r.returncode == 0, r.stderr
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and "THROWN" in r.stdout, r.stdout + r.stderr
+
+
+def test_the_entry_module_runs_as_a_script_too():
+    """`python __graft_entry__.py smoke` calls smoke() from the module's last statement: every name it uses is bound by then."""
+    import ast
+    from pathlib import Path
+    body = ast.parse((Path(__file__).resolve().parent.parent / "__graft_entry__.py").read_text()).body
+    mains = [i for i, node in enumerate(body) if isinstance(node, ast.If) and "__main__" in ast.unparse(node.test)]
+    assert mains == [len(body) - 1]
