@@ -396,7 +396,9 @@ extern "C" int mxk_qkv_norm_rope_append(const MxkAppendArgs* args, const MxkKvCa
   if (rope && (a.rot < 0 || a.rot > cache->D || a.rot % 2 != 0))
     return fail(MXK_ERR_INVALID_ARG, "%s: rot=%d must be even and <= D=%d", name, a.rot, cache->D);
   if (rope && a.rot > 0 && (!a.cos || !a.sin)) return fail(MXK_ERR_INVALID_ARG, "%s: rotary mode needs cos and sin tables", name);
-  p.heads = a.H + 2 * cache->Hkv;
+  const int64_t heads = int64_t(a.H) + 2 * int64_t(cache->Hkv);
+  if (heads >= (int64_t(1) << 30)) return fail(MXK_ERR_TOO_LARGE, "%s: H=%d and Hkv=%d heads", name, a.H, cache->Hkv);
+  p.heads = int(heads);
   p.inv_d = 1.f / float(cache->D);
   p.err = device_error_word();
   const int half = rope ? a.rot / 2 : 0;

@@ -1,5 +1,8 @@
 """Refusals of the attention operators and of the paged cache, checked before anything reaches a GPU."""
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
@@ -90,6 +93,19 @@ def test_append_null_structs_and_noops(L):
     assert lib.mxk_qkv_norm_rope_append(append(L, T=1 << 31), cache(L), None) == -3
     assert lib.mxk_qkv_norm_rope_append(append(L, T=0), None, None) == 0
     assert lib.mxk_qkv_norm_rope_append(append(L, T=-2, q=None), cache(L), None) == 0
+
+
+@pytest.mark.parametrize("D", [72, 128])
+def test_append_refuses_more_heads_than_it_can_count(L, D):
+    """In a process of its own: such a call has ended in a division by zero."""
+    code = f"""import sys; sys.path.insert(0, {str(Path(__file__).parent)!r}); sys.path.insert(0, {str(Path(__file__).parent.parent)!r})
+import test_cpu_attention as t
+from miroxen_b200 import _lib as L
+for H, Hkv in ((2**31 - 1, 2**30), (2**31 - 1, 1), (8, 2**31 - 1), (2**30 - 2, 1)):
+    assert L.lib().mxk_qkv_norm_rope_append(t.append(L, H=H, rot={D}, q_stride=0), t.cache(L, Hkv=Hkv, D={D}, head_stride={D}), None) == -3, (H, Hkv)
+    assert b"qkv_norm_rope_append" in L.lib().mxk_last_error()
+"""
+    subprocess.run([sys.executable, "-c", code], check=True)
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(seq_lens=None), dict(out=None), dict(workspace=None), dict(q=P + 2), dict(out=P + 8),
