@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
   // sequences that have no token in view: out 0, lse -inf
   for (int b = blockIdx.x; b < p.c.n_seqs; b += gridDim.x) {
     if (view_of(p, b).len > 0) continue;
-    for (int i = tid; i < p.a.H * D; i += kThreadsD) p.a.out[int64_t(b) * p.a.H * D + i] = 0;
+    for (int64_t i = tid; i < int64_t(p.a.H) * D; i += kThreadsD) p.a.out[int64_t(b) * p.a.H * D + i] = 0;
     if (p.a.lse)
-      for (int i = tid; i < p.a.H; i += kThreadsD) p.a.lse[int64_t(b) * p.a.H + i] = -INFINITY;
+      for (int64_t i = tid; i < p.a.H; i += kThreadsD) p.a.lse[int64_t(b) * p.a.H + i] = -INFINITY;
   }
   const bool joins = p.cluster > 1 && cur.n_tiles > 0;  // the same for the whole cluster
   if (n_my <= 0 && (!joins || warp >= kWarps)) return;

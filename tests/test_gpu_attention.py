@@ -417,6 +417,21 @@ def test_decode_refuses_a_small_workspace(mx):
     assert bool((out == 7).all())
 
 
+def test_decode_rows_of_more_than_31_bits(mx):
+    """More than 2^31 elements in the heads of one sequence: none of them left out where it is empty, and all of them right where it
+    has one token (its value, whatever the query)."""
+    H, D = (1 << 24) + 3, 128
+    kv = rand(gen(32), 2, 1, 16, 1, D)
+    cache = mx.KvCache(kv[0], kv[1], torch.zeros(2, 1, dtype=torch.int32, device="cuda"))
+    q = torch.zeros(H, D, device="cuda", dtype=torch.bfloat16)
+    out, lse = torch.full((2, H, D), 7.0, device="cuda", dtype=torch.bfloat16), torch.full((2, H), 7.0, device="cuda")
+    mx.attn_decode_paged(q, cache, torch.tensor([0, 1], device="cuda", dtype=torch.int32), H, 0.1, out, q_stride=0, lse=lse, workspace=mx.attn_decode_workspace(cache, H))
+    assert not bool(out[0].view(torch.int64).any()) and bool((lse[0] == -math.inf).all())
+    assert torch.equal(out[1], kv[1, 0, 0].expand(H, D)) and not bool(lse[1].any())
+    del q, out, lse
+    torch.cuda.empty_cache()
+
+
 def test_decode_offsets_past_32_bits(mx):
     g = gen(21)
     pages, page, Hkv, D = 18000, 128, 8, 128  # 2.36e9 elements each
