@@ -608,6 +608,14 @@ def test_window_tiles_in_either_order(mx, order):
     check_window(mx, 53, [9000], [9000], 8, 2, 64, 200, 0, 3, cu=False)
 
 
+@pytest.mark.parametrize("left, right, sinks", [(-1, -1, 0), (-1, 0, 0), (300, 0, 5), (400, 150, 130)])
+@pytest.mark.parametrize("D", [128, 64])
+def test_window_second_tiles(mx, order, D, left, right, sinks):
+    """More tiles than the GPU has CTAs for, of two halves and several blocks each, so that a CTA goes from one to the next: the ring of
+    stages and the queries used again, the next tile's scores under the last one's output."""
+    check_window(mx, 56, [1500, 900, 1211], [1500, 1300, 1211], 24, 8, D, left, right, sinks, behind=3)
+
+
 def test_window_scores_that_grow_along_the_keys(mx):
     """Every block of keys has a larger maximum than the one in front of it, by more and by less than a factor of 2^8."""
     def edit(q, k, v):
@@ -773,6 +781,56 @@ def test_a_prompt_and_then_single_tokens(mx, kind):
             else:  # e4m3: each k and v off by 2^-4 of itself at most (and 2^-10 steps), a score by 2^-4 of its products
                 size = D ** -0.5 * (q1[b].float().abs().view(H, D).amax(1) * torch.stack(keys[b]).float().abs().sum(-1).amax())
                 assert bool(((o1[b].double() - ref[0][0]).norm(dim=1) <= ref[0][0].norm(dim=1) + 4).all()) and bool(size.isfinite().all())
+
+
+def test_single_tokens_over_8_bits_against_what_went_in(mx):
+    """Append into an e4m3 cache and attention over it, against a softmax in 64 bits of the very inputs.  Bounds: a stored key is off by at
+    most 2^-4 of itself and 2^-10 scales (half a step, normal and subnormal), q_out by 2^-8, so a score by d = scale * sum(|q| dk +
+    dq (|k| + dk)), a weight by a factor exp(2 d), and the output by (exp(2 d) - 1) sum w |v| + exp(2 d) sum w dv and the kernel's own
+    roundings.  Queries, keys and values of one sign make the scores and outputs many times as large as that: an output of
+    zero, or of another scale, fails."""
+    g = gen(57)
+    H, Hkv, D, page, left, sinks, steps, ks, vs = 8, 2, 128, 16, 70, 4, 5, 0.02, 0.013
+    start = [100, 37, 1]
+    n, most = len(start), max(start) + steps
+    cache = make_cache(mx, g, E4M3, n, most, page, Hkv, D, fill=False)
+    cache.k_scale.fill_(ks), cache.v_scale.fill_(vs)
+    wq, wk = 0.2 + 0.02 * torch.rand(D, device="cuda", generator=g), 1 + 0.1 * torch.rand(D, device="cuda", generator=g)
+    ws, scale = mx.attn_decode_workspace(cache, H), D ** -0.5
+    keys, vals = [[] for _ in range(n)], [[] for _ in range(n)]
+
+    def append(ids, pos):
+        T = len(ids)
+        q, k = rand(g, T, H, D).abs() + 0.01, rand(g, T, Hkv, D).abs() + 0.01
+        v, q_out = (1 + 0.3 * rand(g, T, Hkv, D)).bfloat16(), torch.empty(T, H, D, device="cuda", dtype=torch.bfloat16)
+        mx.qkv_norm_rope_append(q, k, v, T, H, D, wq, wk, 1e-6, None, None, 0, 0, 0, cache, torch.tensor(pos, dtype=torch.int32).cuda(), q_out,
+                                seq_ids=torch.tensor(ids, dtype=torch.int32).cuda())
+        k64 = R.rope_reference(k, wk, None, None, 0, 0, 1e-6)
+        for t, b in enumerate(ids):
+            keys[b].append(k64[t]), vals[b].append(v[t].double())
+        return q_out, R.rope_reference(q, wq, None, None, 0, 0, 1e-6)
+
+    append([b for b in range(n) for _ in range(start[b])], [t for b in range(n) for t in range(start[b])])
+    for i in range(steps):
+        lens = [m + i + 1 for m in start]
+        q_out, q64 = append(list(range(n)), [m + i for m in start])
+        out, lse = torch.empty_like(q_out), torch.empty(n, H, device="cuda")
+        mx.attn_decode_paged(q_out, cache, torch.tensor(lens, dtype=torch.int32).cuda(), H, scale, out, left=left, sinks=sinks, lse=lse, workspace=ws)
+        own = R.decode_reference(q_out, cache, lens, H, scale, left, sinks)
+        for b, m in enumerate(lens):
+            see = R.visible(1, m, left, 0, sinks, "cuda")[0]
+            for h in range(H):
+                q, k, v = q64[b, h], torch.stack(keys[b])[see, h * Hkv // H], torch.stack(vals[b])[see, h * Hkv // H]
+                s = scale * k @ q
+                w = s.softmax(0)
+                dk, dv, dq = (2.0 ** -4 + 2.0 ** -16) * k + 2.0 ** -10 * ks, 2.0 ** -4 * v.abs() + 2.0 ** -10 * vs, (2.0 ** -8 + 2.0 ** -16) * q
+                d = float((scale * (dk @ q + (k + dk) @ dq)).max())
+                bound = math.expm1(2 * d) * (w @ v.abs()) + math.exp(2 * d) * (w @ dv) + own[2][b, h]
+                want, want_lse = w @ v, torch.logsumexp(s, 0)
+                assert bool(((out[b, h].double() - want).abs() <= bound).all())
+                assert abs(float(lse[b, h].double() - want_lse)) <= d + float(own[3][b, h])
+                # what the bounds would refuse: an output of zero, one of half the values, keys of half their size
+                assert bool((bound < want.abs() / 2).float().mean() > 0.99) and d + float(own[3][b, h]) < float(s.min()) / 2
 
 
 def test_tensors_of_another_place_or_type_are_refused(mx):
