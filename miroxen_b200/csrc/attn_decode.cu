@@ -41,6 +41,7 @@
 #include "bulk_copy.cuh"
 #include "common.cuh"
 #include "kv_cache.cuh"
+#include "tuning.h"
 
 namespace mxk {
 namespace {
@@ -66,6 +67,7 @@ struct DecodeLaunch {
   int ctas;        // runs
   int cluster;     // 0: runs over all tiles; n > 0: the tiles of a work item cut among n CTAs (a cluster where n > 1)
   float scale2;    // scale * log2(e)
+  unsigned tries;       // of a wait for a tile
   unsigned page_recip;  // floor((2^32 - 1) / page_size)
   float* part_o;   // [2 ctas][rows][DP], rows: query heads per block
   float* part_ml;  // [2 ctas][rows][2]
@@ -374,7 +376,8 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       }
       if (i + 1 < n_my) look_up();
       if (i >= kSt) {
-        ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u));
+        // (the computing warps come to their arrival whatever becomes of their own waits, which p.tries bounds)
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&empty[st]), unsigned(i / kSt - 1) & 1u, 0xffffffffu));
         if (!ok) break;
       }
 #pragma unroll
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(kThreadsD) decode_kernel(const __grid_constant
       }
     }
     // A wait that runs out does not leave the loop: the four warps go on meeting, without waiting for anything else.
-    ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&full[st]), ph));
+    ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(smem_u32(&full[st]), ph, p.tries));
     const unsigned k_u = ring_u + unsigned(st) * 2 * Cfg::kTileBytes, v_u = k_u + Cfg::kTileBytes;
 
     // ---- scores of this warp's tokens ----
@@ -899,6 +902,9 @@ int mxk_attn_decode_paged(const MxkDecodeArgs* args, const MxkKvCache* cache, mx
   const int64_t tiles = int64_t(cache->n_seqs) * p.heads * (ceil_div(int64_t(cache->max_pages) * cache->page_size, 64) + 1);
   if (tiles >= (int64_t(1) << 30)) return fail(MXK_ERR_TOO_LARGE, "%s: n_seqs * heads * tokens too large (%lld tiles)", name, (long long)tiles);
   p.scale2 = a.scale * kLog2e;
+  // A warp may have to wait while another passes over sequences without a token, one look at a length each, less than 1.5 us.
+  const int64_t tries = tune(TUNE_DECODE_WAIT_TRIES, int(kSpinTries)) + 4 * int64_t(cache->n_seqs);
+  p.tries = unsigned(tries < 0xffffffffll ? tries : 0xffffffffll);
   p.page_recip = 0xffffffffu / unsigned(cache->page_size);
   p.err = device_error_word();
   const cudaStream_t s = as_stream(stream);

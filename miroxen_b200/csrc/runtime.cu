@@ -21,7 +21,7 @@ const char* const kTuneNames[TUNE_COUNT] = {
     "norm_stages",  "rope_path",        "rope_stages",  "ew_ctas_per_sm",   "res_path",     "rope_tokens",
     "stream_warps", "stream_stages",    "stream_ctas_per_sm", "stream_chunk_kb", "act_path",
     "pdl",          "norm_interleave", "pipe_interleave", "quant_rows_per_cta", "quant_path", "rope_unroll", "rope_wide", "rope_wide_regs", "linear_ctas", "linear_group_m",
-    "window_order", "window_wait_tries",
+    "window_order", "window_wait_tries", "decode_wait_tries",
 };
 }  // namespace
 

@@ -39,6 +39,7 @@ enum TuneKey {
   TUNE_LINEAR_GROUP_M,     // linear layers: row tiles per band of the tile order (default 8 for CTA pairs, 16 for single CTAs)
   TUNE_WINDOW_ORDER,       // attn_window: 1 tiles from the back of the batch (default), 2 from its front
   TUNE_WINDOW_WAIT_TRIES,  // attn_window: tries of a wait between its warps, 1.5 us each, before it counts as run out (default 2^22), beside those that long views add
+  TUNE_DECODE_WAIT_TRIES,  // attn_decode_paged: the same, beside those that many sequences add
   TUNE_COUNT
 };
 

@@ -312,6 +312,32 @@ def test_decode_many_sequences(mx, kind):
     check_decode(mx, 16, kind, [rng.randrange(1, 3000) for _ in range(9)], 16, 2, 128, 64)
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_decode_passes_over_many_empty_sequences(mx, kind):
+    """A run of tiles that ends one sequence and goes on in the next one that has tokens, 200000 empty ones further: a wait between warps,
+    here of 0.8 ms and what the sequences add to it, must not run out meanwhile."""
+    g = gen(33)
+    seqs, Hkv, D, page = 200000, 5, 128, 64
+    cache = make_cache(mx, g, kind, 2, 4224, page, Hkv, D)
+    table = torch.full((seqs, 70), -1, dtype=torch.int32, device="cuda")
+    table[0, :66], table[-1, :66] = cache.page_table[0], cache.page_table[1]
+    wide = mx.KvCache(cache.k, cache.v, table, cache.k_scale, cache.v_scale)
+    q = rand(g, seqs, Hkv * D).view(seqs, Hkv, D)
+    mx.set_tuning("decode_wait_tries", 1 << 9)
+    try:
+        for first in (61 * 64, 62 * 64 - 3, 63 * 64):
+            lens = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+            lens[0], lens[-1] = first, 4160
+            out, lse = torch.full_like(q, 7.0), torch.full((seqs, Hkv), 7.0, device="cuda")
+            mx.attn_decode_paged(q, wide, lens, Hkv, D ** -0.5, out, lse=lse, workspace=mx.attn_decode_workspace(wide, Hkv))
+            want = R.decode_reference(q[[0, -1]], cache, [first, 4160], Hkv, D ** -0.5, -1, 0)
+            R.assert_within(out[[0, -1]], want[0], want[2])
+            R.assert_within(lse[[0, -1]], want[1], want[3])
+            assert not bool(out[1:-1].any()) and bool((lse[1:-1] == -math.inf).all())
+    finally:
+        mx.set_tuning("decode_wait_tries", 0)
+
+
 def test_decode_uneven_scores(mx):
     """A key whose score lies far above all others, late in the sequence: what was summed before it has to vanish."""
     g = gen(17)
