@@ -30,10 +30,12 @@
 // Scores, maxima, sums and output are fp32; probabilities are rounded to bf16 (f16 for an e4m3 cache) for the product, as
 // the tensor instruction needs the type of V.
 //
-// Measured (floor at 6560 GB/s in brackets): 64 sequences of 4100 to 16384 bf16 tokens, 32 heads on 8 of 128, pages of 16:
-// 407 us (382); 8 sequences with 32833 e4m3 tokens in view, 40 heads on 8: 96 us (82); 48 of 2250 to 9000 e4m3 tokens, 28 heads
-// on 4 of 64: 38 us (22 - rows of 64 bytes take as many instructions per token as longer ones: issue slots 59 % used; with the
-// heads outermost in a page the same).
+// Measured in replays on the same inputs (floor at 6560 GB/s in brackets): 64 sequences of 4100 to 16384 bf16 tokens, 32 heads on 8
+// of 128, pages of 16: 407 us (382; 420 in a run with changing inputs); 8 sequences with 32833 e4m3 tokens in view, 40 heads on 8:
+// 95 us (82; 108); 48 of 2250 to 9000 e4m3 tokens, 28 heads on 4 of 64: 38 us (22; 40) - rows of 64 bytes take as many instructions per
+// token as longer ones: issue slots 50 % used, ALU 43 %; with the heads outermost in a page the same.
+// Blocks of 16 heads, 64 sequences of 4100 to 16384 tokens, 2 key heads of 128 (bf16: 106, e4m3: 53): 8 heads on each 120 and 84 us, 12
+// heads 122 and 78, 16 heads 124 and 80, 32 heads, two blocks, which read the cache one after the other, 214 and 146.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -251,6 +253,8 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
 //   as many CTAs as there are registers for to the other e4m3 rows (8 sequences with 32832 tokens in view, D = 128: 95 us with two
 //   stages, 102.5 with three or four, 112 with LONG tiles), which take more arithmetic per byte, and to short calls, where a CTA has
 //   few tiles (300 sequences of 600 tokens, 4 heads of 64: e4m3 22 us against 28, bf16 30 against 34 with LONG tiles).
+// Chosen with blocks of 8 heads.  Blocks of 16 take the same for want of a case where it counts for more: D = 128, 32 heads on 2, 64
+// sequences of up to 16384 tokens, bf16 124 us with three stages, 123 with two or four; e4m3 80 with two, 77.5 with three or four.
 template <bool E4M3, int DP, bool LONG>
 struct DecodeCfg {
   static_assert(!LONG || DP == 64, "LONG tiles belong to short rows");
@@ -832,7 +836,7 @@ int launch_decode(const char* name, DecodeLaunch& p, cudaStream_t s) {
   };
   if (ceil_div(short_tiles, c) <= (2 * items >= 3 * resident ? kMedium : kShort) && items * c < (int64_t(1) << 31)) return one_launch(Int<0>());
   // Whole items of LONG tiles where those have two CTAs per SM to fill: 200 sequences of 2000 e4m3 tokens, 4 heads of 64, 42 against
-  // 52 us by runs, of 4000 73 against 100; bf16 54 and 97 against 53 and 98.
+  // 52 us by runs, of 4000 73 against 100; bf16, the same either way (54 and 97 against 53 and 98), follows the rule.
   if constexpr (kLong) {
     c = 1;
     if (item_tiles <= kMedium && 2 * items >= 3 * int64_t(decode_ctas<E4M3, DP, NH, true>()) && items < (int64_t(1) << 31)) return one_launch(Int<1>());

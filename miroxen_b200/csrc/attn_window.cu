@@ -28,10 +28,10 @@
 // output that is not finite has its rows' edge blocks looked through, and if it can have come from there the row is taken
 // again by a plain loop (row_attention) that never touches what the row does not see.
 //
-// Measured (D = 128): 2 x 4352 rows x 24 heads, everything visible, 360 us = 1290 TFLOP/s from a cold start, 429 us = 1085
+// Measured (D = 128): 2 x 4352 rows x 24 heads, everything visible, 361 us = 1290 TFLOP/s from a cold start, 420 us = 1108
 // TFLOP/s in a run of seconds, where the power limit holds the clock near 1530 MHz (a library product: 1651 and 1393);
 // 33272 rows x 5 heads with a window of 6240 each way and 1560 first keys 800 us; nine packed causal prompts of 14 to 3414 rows,
-// 32 heads on 8, window 1024: 113 us; one prompt of 77 rows: 6.9 us.  What bounds it: the tensor pipe, busy 69 % of the time
+// 32 heads on 8, window 1024: 114 us; one prompt of 77 rows: 6.8 us.  Heads of 72 or 80 take products of 128: 336 us for the first case.  What bounds it: the tensor pipe, busy 69 % of the time
 // (the scores' operands both come from shared memory, 98 clocks instead of 64 per product), and the last round of tiles.
 #include <cuda.h>
 
